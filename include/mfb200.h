@@ -283,6 +283,139 @@ MFB200_API int mfb200_splitk_gemm_noalloc(const void *d_A, const void *d_W, int 
                                           int k_splits, const float *d_bias, float *d_out,
                                           void *stream);
 MFB200_API const char *mfb200_noalloc_last_error(void);
+
+/* ---- Operators on policy logits and legal-move lists (device buffers) ----
+ *
+ * For programs that score or tune a policy on the device: log-probabilities
+ * over the legal moves with their backward pass, a clipped policy loss with a
+ * KL term, and a preference loss over lines of moves, the losses with their
+ * gradients. No counterpart in the reference, whose leaf step stops at the
+ * priors (mfb200_evaluate_priors). They read what that step reads: one row of
+ * policy logits for each position (what mfb200_evaluate_device writes, or a
+ * trainer's own) and the legal moves as a CSR list of policy indices.
+ *
+ * Every pointer named d_* and every pointer of mfb200_policy_rows is a device
+ * pointer of the current device (the logits' device is checked); the work is
+ * enqueued on `stream` (a cudaStream_t, NULL = legacy default stream) without
+ * synchronising. The calls allocate nothing, keep nothing between calls and
+ * can be captured into a CUDA graph; calls on different streams or threads do
+ * not share anything but the buffers they are given. Results do not depend on
+ * timing: the same inputs give the same bits. Returns 0 on success;
+ * mfb200_policy_last_error() gives the calling thread's last message.
+ *
+ * The softmax of a position runs over its first n = min(count, 256) listed
+ * moves (as in mfb200_evaluate_priors): s_j = logit[move_index_j] /
+ * softmax_temp, logp_j = s_j - log(sum exp s). An index outside [0, classes)
+ * counts as logit 0 and gets no gradient; an index that is listed twice counts
+ * twice, and its column gets the sum of both gradients. Columns that are not
+ * listed are never read, whatever they hold. A position without a legal move
+ * (empty list, or every listed logit -inf) takes part in nothing: zero losses,
+ * zero gradients, log-probability 0 for its played move and -inf for listed
+ * ones. A NaN or +inf among the listed logits makes the position's results
+ * NaN. A position whose offsets decrease or reach outside [0, num_moves], or
+ * whose played move is below -1 or not among its n moves, is not read past its
+ * list: its per-position results and its whole gradient row are NaN. Sums and
+ * softmax statistics are 32-bit or wider whatever the logits' type; each
+ * gradient is rounded once to its own type. */
+
+/* Element types of matrices of logits and of their gradients. */
+enum { MFB200_TYPE_F32 = 0, MFB200_TYPE_BF16 = 1, MFB200_TYPE_F16 = 2 };
+
+typedef struct {
+  const void *logits;          /* [batch, classes], rows logits_stride elements apart */
+  int64_t logits_stride;       /* >= classes */
+  int32_t logits_type;         /* MFB200_TYPE_* */
+  int32_t batch;               /* positions; 0 does nothing */
+  int32_t classes;             /* columns of a row, 1..32767 (1858 for this library's networks) */
+  const int32_t *move_offsets; /* [batch + 1]; position b's moves are move_index
+                                  [move_offsets[b] - move_offsets[0], move_offsets[b + 1] - move_offsets[0]) */
+  const int16_t *move_index;   /* [num_moves] policy index of each legal move */
+  int64_t num_moves;
+  const int32_t *played;       /* [batch] the played move's place in its position's list; -1: none (a
+                                  padded position, the other side's move). May be NULL where it is not used */
+  double softmax_temp;
+} mfb200_policy_rows;
+
+/* d_move_logp [num_moves]: log-probability of each listed move (-inf past the
+ * 256th); entries that no position lists are left as they are. d_played_logp
+ * [batch]: of the played move, 0 where there is none. d_entropy [batch]:
+ * -sum p log p. Each may be NULL, but not all. */
+MFB200_API int mfb200_move_logprobs(const mfb200_policy_rows *rows, float *d_move_logp,
+                                    float *d_played_logp, float *d_entropy, void *stream);
+
+/* Backward pass of mfb200_move_logprobs: from the gradients of its outputs
+ * (d_grad_moves [num_moves], d_grad_played [batch], d_grad_entropy [batch];
+ * a NULL one is zero) the gradient of the logits, [batch, classes] with rows
+ * grad_stride elements apart in grad_type. All columns are written (0 for
+ * moves that are not listed); elements between the rows are left as they are.
+ * With d_grad_moves = -target this is the gradient of the cross-entropy to a
+ * distribution over the legal moves, such as the search's visit counts. The
+ * gradient may not overlap an input. */
+MFB200_API int mfb200_move_logprobs_backward(const mfb200_policy_rows *rows,
+                                             const float *d_grad_moves, const float *d_grad_played,
+                                             const float *d_grad_entropy, void *d_grad_logits,
+                                             int64_t grad_stride, int grad_type, void *stream);
+
+typedef struct {
+  double clip_low, clip_high; /* the ratio is clipped to [1 - clip_low, 1 + clip_high] */
+  float kl_coef;              /* weight of KL(policy || reference) */
+  float entropy_coef;         /* weight of the entropy, which is subtracted */
+  float scale;                /* of every loss and gradient: 1 / batch for a mean */
+} mfb200_clip_config;
+
+/* Clipped policy loss with a KL term, and its gradient, in one pass. For the
+ * played move's probability ratio r = exp(logp - d_old_logp[b]) and the
+ * position's d_advantage A:
+ *   loss[b] = scale * weight[b] * ( -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *             + kl_coef * KL - entropy_coef * H ),
+ * KL = sum p (log p - log q) over the legal moves against the softmax q of
+ * d_ref_logits ([batch, classes], rows ref_stride apart, ref_type; same
+ * softmax_temp; NULL for no KL term), H the entropy. d_weight NULL means 1. A
+ * position without a played move has loss 0 and a zero gradient. The clip is
+ * decided in 64 bits; at its border the gradient is the unclipped one.
+ * Outputs, each may be NULL: d_loss, d_logp (0 without a played move), d_kl,
+ * d_entropy [batch]; d_total [1], the sum of d_loss (needs d_loss);
+ * d_grad_logits as in mfb200_move_logprobs_backward. A reference logit of -inf
+ * at a move that the policy gives a probability makes the KL infinite. */
+MFB200_API int mfb200_clipped_policy_loss(const mfb200_policy_rows *rows,
+                                          const mfb200_clip_config *cfg, const float *d_old_logp,
+                                          const float *d_advantage, const float *d_weight,
+                                          const void *d_ref_logits, int64_t ref_stride,
+                                          int ref_type, float *d_loss, float *d_logp, float *d_kl,
+                                          float *d_entropy, float *d_total, void *d_grad_logits,
+                                          int64_t grad_stride, int grad_type, void *stream);
+
+typedef struct {
+  float beta;            /* of the margin */
+  float label_smoothing; /* probability that a pair is the wrong way round, 0..1 */
+  float scale;           /* of every loss and gradient: 1 / pairs for a mean */
+} mfb200_preference_config;
+
+/* Preference loss (paired log ratios) over lines of moves, and its gradient.
+ * A line is a run of positions of the batch with their played moves:
+ * d_line_offsets [2 * pairs + 1] into the positions, non-decreasing; line 2i
+ * is the preferred and 2i + 1 the rejected one of pair i. With d_ref_logp
+ * [batch] the reference policy's log-probability of each played move
+ * (mfb200_move_logprobs on its logits) and D = the sum of logp - ref_logp over
+ * a line's positions that have a played move:
+ *   margin[i] = beta * (D_preferred - D_rejected),
+ *   loss[i] = scale * weight[i] * ( -(1 - eps) log sigma(margin) - eps log sigma(-margin) ).
+ * A line may be empty (D = 0); positions in no line get a zero gradient. A
+ * pair whose offsets decrease or leave the batch has NaN results. d_weight
+ * NULL means 1. Written: d_logp [batch], d_row_grad [batch] (the gradient of
+ * the total with respect to d_logp), d_line_logp [2 * pairs], d_margin, d_loss
+ * [pairs]; optional d_total [1] and d_grad_logits as in
+ * mfb200_move_logprobs_backward. */
+MFB200_API int mfb200_preference_loss(const mfb200_policy_rows *rows,
+                                      const mfb200_preference_config *cfg,
+                                      const int32_t *d_line_offsets, int pairs,
+                                      const float *d_ref_logp, const float *d_weight,
+                                      float *d_logp, float *d_row_grad, float *d_line_logp,
+                                      float *d_margin, float *d_loss, float *d_total,
+                                      void *d_grad_logits, int64_t grad_stride, int grad_type,
+                                      void *stream);
+MFB200_API const char *mfb200_policy_last_error(void);
+
 MFB200_API void mfb200_destroy(mfb200_handle *h);
 
 #ifdef __cplusplus

@@ -1,0 +1,30 @@
+// policy.cuh -- operators on policy logits and legal-move lists (policy.cu).
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace mfb200 {
+
+// A batch of policy rows with their legal moves, on the device (the fields of
+// mfb200_policy_rows; off[0] is the position of index[0]).
+struct PolicyRows {
+  const void *logits;
+  long long stride;  // elements between rows
+  int type;          // MFB200_TYPE_*
+  int batch, classes;
+  const int32_t *off;     // [batch + 1]
+  const int16_t *index;   // [num_moves]
+  long long num_moves;
+  const int32_t *played;  // [batch] edge numbers, or null
+  double temp;
+  float inv_temp;
+};
+
+// Log-probabilities of the legal moves, of the played move and the entropy;
+// each output may be null. row_state, if set, receives +0 for rows that take
+// part in a loss and -0 for rows that do not (see preference_pair_kernel).
+cudaError_t launch_move_logprobs(const PolicyRows &r, float *move_logp, float *played_logp,
+                                 float *entropy, float *row_state, cudaStream_t s);
+
+}  // namespace mfb200
