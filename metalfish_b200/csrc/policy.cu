@@ -12,24 +12,30 @@
 //
 // What bounds them. The arithmetic is ~40 operations a move: nothing. The
 // log-probabilities read one 32-byte sector of the row for almost every move
-// (19 sectors for the 31 moves of an average position) in three dependent
-// steps (offsets, indices, logits), so they are bound by load latency until
-// the sectors' bandwidth. The gradient operators are bound by writing the
-// whole row (1858 x 4 bytes), 8 times what they read.
+// (19 sectors for the 31 moves of an average position, 64 bytes of DRAM each)
+// in three dependent steps (offsets, indices, logits), so they are bound by
+// load latency and by the instructions of a row, not by its bytes. The gradient
+// operators write the whole row (1858 x 4 bytes), 8 times what they need to
+// read: they are bound by DRAM writes.
 //
-// One warp per position: a lane holds up to eight moves in registers, the
-// sums are shuffles in a fixed order (results do not depend on timing), and
-// nothing goes through shared memory but the test for repeated indices. The
-// zeros of a gradient row are stored first, as 16-byte pieces, so that they
-// drain while the warp waits for its three loads; the ~30 values follow after
-// a __syncwarp and meet the zeros in L2.
+// One warp per position: a lane holds two moves in registers, the sums are
+// shuffles in a fixed order (results do not depend on timing). CTAs stay on
+// their SM and their warps take positions in turn, the lists of the next ones
+// loaded ahead. A gradient row is put together in shared memory and written by
+// one bulk copy, while the warp goes on. 65536 positions, 1858 fp32 classes, on
+// B200: clipped loss with KL 136 us (615 MB of DRAM traffic, 4.5 TB/s; the
+// copies of empty lists alone 75 us), its backward pass alone 102 us,
+// log-probabilities 35 us.
 #include "policy.cuh"
 
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 
 #include "../../include/mfb200.h"
+#include "gemm_host.h"  // num_sms
 #include "pdl.cuh"
+#include "sm100_ptx.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -40,31 +46,39 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kMaxMoves = 256;  // moves of a position that count, as in priors_kernel
-constexpr int kPerLane = kMaxMoves / 32;
-constexpr int kMaxWarps = 8;  // positions per CTA
+constexpr int kMaxWarps = 8;    // positions per CTA at a time
+constexpr float kLog2e = 1.4426950408889634f;
 
-// One iteration for each group of 32 moves that the position has; n is the
-// same in every lane, so the groups past it are skipped by the whole warp.
-// Inputs are read with ordinary loads, never as read-only (__ldg, __restrict__
-// const): a kernel here may start before the one that writes its inputs has
-// ended (pdl.cuh), and a read-only load may be moved above pdl_wait.
-#define FOR_GROUPS(k, n) _Pragma("unroll") for (int k = 0; k < kPerLane; ++k) if (32 * k < (n))
+// Inputs are read with ordinary or volatile loads, never as read-only (__ldg,
+// __restrict__ const): a kernel here may start before the one that writes its
+// inputs has ended (pdl.cuh), and a read-only load may be moved above pdl_wait.
 
-__device__ __forceinline__ float load_as_float(const void *base, int type, long long i) {
-  if (type == MFB200_TYPE_F32) return static_cast<const float *>(base)[i];
-  const unsigned short u = static_cast<const unsigned short *>(base)[i];
+// A logit. L2 takes 64 bytes from DRAM for it instead of the 128 that a plain
+// load takes: 65536 gathers of 16 pairs of logits a row read 88 MB instead of
+// 155, in 17.4 instead of 26.5 us.
+__device__ __forceinline__ float load_logit(const void *row, int type, int c) {
+  if (type == MFB200_TYPE_F32) {
+    float v;
+    asm volatile("ld.global.L2::64B.f32 %0, [%1];" : "=f"(v) : "l"(static_cast<const float *>(row) + c));
+    return v;
+  }
+  unsigned short u;
+  asm volatile("ld.global.L2::64B.u16 %0, [%1];"
+               : "=h"(u)
+               : "l"(static_cast<const unsigned short *>(row) + c));
   return type == MFB200_TYPE_BF16 ? __uint_as_float(static_cast<unsigned>(u) << 16)
                                   : __half2float(__ushort_as_half(u));
 }
 
+__device__ __forceinline__ const void *row_of(const void *base, int type, long long stride, int b) {
+  return static_cast<const char *>(base) + b * stride * (type == MFB200_TYPE_F32 ? 4 : 2);
+}
+
 // One rounding, to nearest even, of the fp32 value to the gradient's type.
-__device__ __forceinline__ void store_as(void *base, int type, long long i, float v) {
-  if (type == MFB200_TYPE_F32)
-    static_cast<float *>(base)[i] = v;
-  else if (type == MFB200_TYPE_BF16)
-    static_cast<__nv_bfloat16 *>(base)[i] = __float2bfloat16_rn(v);
-  else
-    static_cast<__half *>(base)[i] = __float2half_rn(v);
+__device__ __forceinline__ unsigned bits_of(int type, float v) {
+  if (type == MFB200_TYPE_F32) return __float_as_uint(v);
+  if (type == MFB200_TYPE_BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  return __half_as_ushort(__float2half_rn(v));
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -77,280 +91,581 @@ __device__ __forceinline__ double warp_sum(double v) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   return v;
 }
+// The largest value of the warp; NaN is passed over.
 __device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+  float top;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(v));
+  return top;
+}
+__device__ __forceinline__ float exp2_fast(float t) {
+  float v;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(v) : "f"(t));
   return v;
 }
+__device__ __forceinline__ float quiet_nan() { return __int_as_float(0x7FC00000); }
 
-// A position's legal moves, spread over the warp: move 32 k + lane.
-struct Moves {
-  int n;        // moves that count (<= 256)
-  int count;    // moves listed
-  long long lo; // first entry of the list
-  int played;   // edge number, -1 for none
-  bool bad;     // offsets or played move out of range
-  int col[kPerLane];  // column, -1 for none (the logit is then 0, without a gradient)
-};
-
-// What a list is read with. Loaded first; the zeros of a gradient row are
-// stored between this and the list itself, while these loads are under way.
+// ------------------------------------------------------------------ lists
+// What a position's list is read with.
 struct ListHead {
-  int base, lo, hi, played;
+  int lo, hi, played;
 };
 __device__ __forceinline__ ListHead load_head(const PolicyRows &r, int b) {
-  return {r.off[0], r.off[b], r.off[b + 1], r.played ? r.played[b] : -1};
+  return {r.off[b], r.off[b + 1], r.played ? r.played[b] : -1};
 }
 
-// The list itself. No entry outside [0, num_moves) is read.
-__device__ __forceinline__ Moves load_moves(const PolicyRows &r, const ListHead &head, int lane) {
+struct Moves {
+  int n;       // moves that count (<= 256)
+  int count;   // moves listed
+  int lo;      // first entry of the list
+  int played;  // edge number, -1 for none
+  bool bad;    // offsets or played move out of range
+};
+// No entry outside [0, num_moves) is ever read.
+__device__ __forceinline__ Moves resolve(const PolicyRows &r, const ListHead &head, int base) {
   Moves m;
-  const long long lo = static_cast<long long>(head.lo) - head.base;
-  const long long hi = static_cast<long long>(head.hi) - head.base;
+  const long long lo = static_cast<long long>(head.lo) - base;
+  const long long hi = static_cast<long long>(head.hi) - base;
   m.bad = lo < 0 || hi < lo || hi > r.num_moves;
+  m.lo = m.bad ? 0 : static_cast<int>(lo);
   m.count = m.bad ? 0 : static_cast<int>(hi - lo);
   m.n = m.count < kMaxMoves ? m.count : kMaxMoves;
-  m.lo = lo;
   // a position with an empty list has no played move, whatever it is given
   m.bad = m.bad || head.played < -1 || (m.count > 0 && head.played >= m.n);
   m.played = m.bad || m.count == 0 ? -1 : head.played;
-#pragma unroll
-  for (int k = 0; k < kPerLane; ++k) m.col[k] = -1;
-  FOR_GROUPS(k, m.n) {
-    const int j = 32 * k + lane;
-    if (j < m.n) {
-      const int c = r.index[m.lo + j];
-      m.col[k] = c >= 0 && c < r.classes ? c : -1;
-    }
-  }
   return m;
 }
 
-// Softmax statistics of a row over its list. The largest entry is kept out of
-// the sum (S = 1 + rest), so that log S and 1 - p of a nearly certain move
-// keep their digits.
-struct Norm {
-  float top;    // largest logit
-  float rest;   // sum of exp(s - s_top) over the other moves
-  float log_s, inv_s;
-  int lead;     // lowest edge with the largest logit
-  bool live;    // some move has a logit above -inf (or NaN)
+// Lane's entry of the group of 32 moves k of a list, -1 past its end or for a
+// column outside the row (whose logit is then 0, without a gradient).
+constexpr int kNoMove = -2, kNoColumn = -1;
+__device__ __forceinline__ int load_index(const PolicyRows &r, const Moves &m, int k, int lane) {
+  const int j = 32 * k + lane;
+  return j < m.n ? r.index[m.lo + j] : -32768;
+}
+
+// Runs body(b, moves, first, second) for the positions of this CTA, a warp for
+// each: `first` and `second` are the lane's entries of the first two groups of
+// the list. A CTA has the positions at W = its warps in a row, every grid * W;
+// its warps take them in turn from a counter in shared memory. The list of the
+// next position and the offsets of the one after are loaded while a position
+// is worked on, so of the three loads that follow from one another (offsets,
+// list, logits) only the last is waited for.
+//
+// body may turn a position down by returning true: rare(b, moves) then has it,
+// outside the loop that body is in. What is rare and needs many registers
+// (lists of more than 64 moves, one in a hundred; 64-bit functions) goes
+// there, so that it does not share them with the common path: a spill in that
+// path costs more than its bytes, because the fence before a row's copy waits
+// for it too (65536 positions of the clipped loss took 330 us with 280 bytes
+// of spills). The other warps take the positions that this one is late for.
+template <class Body, class Rare>
+__device__ __forceinline__ void for_positions(const PolicyRows &r, unsigned ctas, unsigned *next_turn,
+                                              Body body, Rare rare) {
+  const int lane = threadIdx.x & 31;
+  const unsigned batch = r.batch;
+  const unsigned warps = blockDim.x >> 5, shift = __popc(warps - 1);  // a power of two
+  const unsigned step = ctas * warps;
+  auto row = [&](unsigned turn) {
+    return blockIdx.x * warps + (turn & (warps - 1)) + (turn >> shift) * step;
+  };
+  const int base = r.off[0];
+  // turns of this warp: now, next, after (the first three are fixed)
+  unsigned t0 = threadIdx.x >> 5, t1 = t0 + warps, t2 = t1 + warps;
+  while (row(t0) < batch) {
+    Moves m = resolve(r, load_head(r, row(t0)), base);
+    ListHead next{};
+    if (row(t1) < batch) next = load_head(r, row(t1));
+    int c0 = load_index(r, m, 0, lane), c1 = m.n > 32 ? load_index(r, m, 1, lane) : -32768;
+    unsigned b;
+    bool turned_down;
+    while (true) {
+      b = row(t0);
+      Moves mn{};
+      int n0 = -32768, n1 = -32768;
+      ListHead after{};
+      if (row(t1) < batch) {
+        mn = resolve(r, next, base);
+        n0 = load_index(r, mn, 0, lane);
+        if (mn.n > 32) n1 = load_index(r, mn, 1, lane);
+        if (row(t2) < batch) after = load_head(r, row(t2));
+      }
+      unsigned t3 = 0;
+      if (lane == 0) t3 = atomicAdd(next_turn, 1u);
+      turned_down = body(static_cast<int>(b), m, c0, c1);
+      t0 = t1;
+      t1 = t2;
+      t2 = __shfl_sync(kFull, t3, 0);
+      if (turned_down || row(t0) >= batch) break;
+      m = mn;
+      c0 = n0;
+      c1 = n1;
+      next = after;
+    }
+    if (turned_down) rare(static_cast<int>(b), resolve(r, load_head(r, b), base));
+  }
+}
+// Sets the counter behind the fixed turns; all threads of the CTA.
+__device__ __forceinline__ void start_turns(unsigned *next_turn) {
+  if (threadIdx.x == 0) *next_turn = 3 * (blockDim.x >> 5);
+  __syncthreads();
+}
+
+// ------------------------------------------------------------------ softmax of a list
+// The moves of a position, 32 k + lane in group k. Lanes past the list's end
+// hold a logit of -inf, which no sum sees.
+template <int G>
+struct Edges {
+  int col[G];
+  float z[G];  // logits
+  float e[G];  // exp(s - s_top)
 };
 
-// z[k]: the logits of the lane's moves. On return e[k] = exp(s - s_top).
-__device__ __forceinline__ Norm normalise(const Moves &m, const float (&z)[kPerLane],
-                                          float inv_temp, int lane, float (&e)[kPerLane]) {
+template <int G>
+__device__ __forceinline__ void columns(const PolicyRows &r, const Moves &m, int c0, int c1,
+                                        int lane, Edges<G> &v) {
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+    int c = k == 0 ? c0 : k == 1 ? c1 : -32768;
+    if (k > 1 && 32 * k < m.n) c = load_index(r, m, k, lane);
+    v.col[k] = c >= 0 && c < r.classes ? c : 32 * k + lane < m.n ? kNoColumn : kNoMove;
+  }
+}
+
+// z[k] from a row of logits; groups past the list's end are not loaded.
+template <int G>
+__device__ __forceinline__ void load_logits(const Moves &m, const void *row, int type,
+                                            const int (&col)[G], float (&z)[G]) {
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+    z[k] = col[k] == kNoMove ? -INFINITY : 0.0f;
+    if (32 * k < m.n && col[k] >= 0) z[k] = load_logit(row, type, col[k]);
+  }
+}
+
+// Softmax statistics. The largest entry is kept out of the sum (S = 1 + rest),
+// so that log S and 1 - p of a nearly certain move keep their digits.
+struct Norm {
+  float top;   // largest logit
+  int lead;    // lowest edge that has it
+  bool live;   // some move has a logit above -inf (or NaN)
+  float rest;  // sum of exp(s - s_top) over the other moves
+  float log_s, inv_s;
+};
+
+// Largest logit, and e[k] = exp(s - s_top) with this lane's part of `rest` and
+// of sum e s. The exponential is 2^(s log2 e) in one instruction; the rounding
+// of its argument, half a step times |s|, is no more than that of s itself.
+template <int G>
+__device__ __forceinline__ Norm softmax_part(int n, const float (&z)[G], float inv_temp,
+                                             float inv_temp2, int lane, float (&e)[G],
+                                             float &es) {
   Norm q;
-  float top = -INFINITY;
-  bool some = false;
-  FOR_GROUPS(k, m.n) {
-    if (32 * k + lane < m.n) {
-      top = fmaxf(top, z[k]);
-      some |= !(z[k] == -INFINITY);
+  float top = z[0];
+#pragma unroll
+  for (int k = 1; k < G; ++k)
+    if (32 * k < n) top = fmaxf(top, z[k]);
+  q.top = warp_max(top);
+  q.live = q.top > -INFINITY;
+  if (!q.live) {
+    bool nan = false;
+#pragma unroll
+    for (int k = 0; k < G; ++k) nan |= 32 * k < n && z[k] != z[k];
+    q.live = __any_sync(kFull, nan);
+  }
+  q.lead = -1;
+  q.rest = 0.0f;
+  es = 0.0f;
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+    e[k] = 0.0f;
+    if (32 * k < n) {
+      const unsigned at = __ballot_sync(kFull, z[k] == q.top);
+      if (q.lead < 0 && at) q.lead = 32 * k + __ffs(at) - 1;
+      const float d = z[k] - q.top;
+      e[k] = exp2_fast(d * inv_temp2);
+      if (e[k] != 0.0f) es += e[k] * (d * inv_temp);
+      if (32 * k + lane != q.lead) q.rest += e[k];
     }
   }
-  q.top = warp_max(top);
-  q.live = __any_sync(kFull, some);
-  q.lead = -1;
-  float rest = 0.0f;
-  FOR_GROUPS(k, m.n) {
-    const bool mine = 32 * k + lane < m.n;
-    const unsigned at = __ballot_sync(kFull, mine && z[k] == q.top);
-    if (q.lead < 0 && at) q.lead = 32 * k + __ffs(at) - 1;
-    e[k] = mine ? expf((z[k] - q.top) * inv_temp) : 0.0f;
-    if (32 * k + lane != q.lead) rest += e[k];
-  }
-  // the largest entry's own inf - inf is not in the sum
-  q.rest = q.top == INFINITY ? __int_as_float(0x7FC00000) : warp_sum(rest);
-  q.log_s = log1pf(q.rest);
-  q.inv_s = 1.0f / (1.0f + q.rest);
   return q;
 }
 
-__device__ __forceinline__ void load_logits(const PolicyRows &r, const Moves &m, const void *base,
-                                            long long stride, int type, int b,
-                                            float (&z)[kPerLane]) {
-  const long long row = static_cast<long long>(b) * stride;
-  FOR_GROUPS(k, m.n) z[k] = m.col[k] >= 0 ? load_as_float(base, type, row + m.col[k]) : 0.0f;
+__device__ __forceinline__ float reciprocal(float x) {
+  float v;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(v) : "f"(x));  // within one step
+  return v;
 }
 
-// The value that move j's lane holds in group v[j / 32].
-__device__ __forceinline__ float of_move(const float (&v)[kPerLane], int n, int j) {
-  float got = 0.0f;
-  FOR_GROUPS(k, n) {
-    const float t = __shfl_sync(kFull, v[k], j & 31);
-    if (j >> 5 == k) got = t;
+// Ends softmax_part for a row and, with kSecond, for a second softmax w over
+// the same list: the sums over the warp, their logarithms and reciprocals.
+// Returns the entropy -sum p log p = log S - sum(e s) / S, two terms that are
+// never negative; `more` is summed as well.
+//
+// The sums share one reduction: after the step over 16 lanes the lower half
+// works on one pair of values and the upper on the other, after the step over
+// 8 each quarter on one, so four sums take 6 shuffles instead of 20, and one
+// logarithm and one reciprocal serve both softmaxes.
+template <bool kSecond>
+__device__ __forceinline__ float softmax_done(Norm &q, float es, Norm &w, float &more, int lane) {
+  const bool upper = lane & 16, second = lane & 8;
+  if (q.top == INFINITY) q.rest = quiet_nan();  // its own inf - inf is not in the sum
+  if (kSecond && w.top == INFINITY) w.rest = quiet_nan();
+  const float x = kSecond ? w.rest : more;
+  float a = (upper ? x : q.rest) + __shfl_xor_sync(kFull, upper ? q.rest : x, 16);
+  float b = es + __shfl_xor_sync(kFull, es, 16);
+  float v = (second ? b : a) + __shfl_xor_sync(kFull, second ? a : b, 8);
+  v += __shfl_xor_sync(kFull, v, 4);
+  v += __shfl_xor_sync(kFull, v, 2);
+  v += __shfl_xor_sync(kFull, v, 1);
+  // lanes 0-7 hold q.rest, 16-23 w.rest or `more`, the others es
+  const float log_v = log1pf(v), inv_v = reciprocal(1.0f + v);
+  q.rest = __shfl_sync(kFull, v, 0);
+  q.log_s = __shfl_sync(kFull, log_v, 0);
+  q.inv_s = __shfl_sync(kFull, inv_v, 0);
+  es = __shfl_sync(kFull, v, 8);
+  if (kSecond) {
+    w.log_s = __shfl_sync(kFull, log_v, 16);
+    w.inv_s = __shfl_sync(kFull, inv_v, 16);
+  } else {
+    more = __shfl_sync(kFull, v, 16);
   }
-  return got;
+  return q.log_s - es * q.inv_s;
 }
 
+// The value of move j, which every lane gets.
+template <int G>
+__device__ __forceinline__ float of_move(const float (&v)[G], int j) {
+  float t = v[0];
+#pragma unroll
+  for (int k = 1; k < G; ++k) t = j >> 5 == k ? v[k] : t;
+  return __shfl_sync(kFull, t, j & 31);
+}
+
+// ------------------------------------------------------------------ gradient rows
 struct Grad {
   void *base;  // null: no gradient
   long long stride;
   int type;
 };
 
-// The row's bytes, all the same element: 16-byte stores between the first and
-// last 16-byte boundary, single elements around them.
-__device__ __forceinline__ void fill_row(const Grad &g, int classes, int b, int lane,
-                                         unsigned word) {
-  const int size = g.type == MFB200_TYPE_F32 ? 4 : 2;
-  char *p = static_cast<char *>(g.base) + static_cast<long long>(b) * g.stride * size;
-  const int bytes = classes * size;
-  int head = static_cast<int>((16 - (reinterpret_cast<unsigned long long>(p) & 15)) & 15);
-  if (head > bytes) head = bytes;
-  const int body = (bytes - head) >> 4;
-  const int tail = head + (body << 4);
-  uint4 v = make_uint4(word, word, word, word);
-  uint4 *q = reinterpret_cast<uint4 *>(p + head);
-  for (int i = lane; i < body; i += 32) q[i] = v;
-  const int around = (head + bytes - tail) / size;
-  if (lane < around) {
-    const int at = lane * size < head ? lane * size : tail + lane * size - head;
-    if (size == 4)
-      *reinterpret_cast<unsigned *>(p + at) = word;
-    else
-      *reinterpret_cast<unsigned short *>(p + at) = static_cast<unsigned short>(word);
+// A warp's gradient row in shared memory, zero between rows. The values of a
+// row's moves are put into it, one bulk copy (cp.async.bulk) writes the whole
+// row, and the values are taken out again before the next row's go in, by
+// which time the copy has read them. The row keeps its place within 16 bytes,
+// so that the copy runs from the first to the last 16-byte boundary of the
+// row; the elements around them are stored singly.
+struct RowImage {
+  char *buf;     // 16-byte aligned, a row and 16 bytes long
+  bool pending;  // a bulk copy may still be reading it
+  int old[2];    // byte offsets of the lane's values, -1 for none
+};
+
+__device__ __forceinline__ size_t image_bytes(int row_bytes) { return ((row_bytes + 127) & ~127) + 128; }
+
+__device__ __forceinline__ RowImage clear_image(char *buf, int row_bytes, int lane) {
+  const int n = static_cast<int>(image_bytes(row_bytes) >> 4);
+  for (int i = lane; i < n; i += 32) reinterpret_cast<uint4 *>(buf)[i] = make_uint4(0, 0, 0, 0);
+  __syncwarp();
+  return {buf, false, {-1, -1}};
+}
+
+__device__ __forceinline__ void put(char *p, int size, unsigned bits) {
+  if (size == 4)
+    *reinterpret_cast<unsigned *>(p) = bits;
+  else
+    *reinterpret_cast<unsigned short *>(p) = static_cast<unsigned short>(bits);
+}
+__device__ __forceinline__ unsigned get(const char *p, int size) {
+  return size == 4 ? *reinterpret_cast<const unsigned *>(p) : *reinterpret_cast<const unsigned short *>(p);
+}
+
+__device__ __forceinline__ void take_out(RowImage &im, int size, int lane) {
+  if (im.pending) {
+    if (lane == 0) bulk_wait_read0();
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (im.old[k] >= 0) put(im.buf + im.old[k], size, 0u);
+    __syncwarp();
+    im.pending = false;
   }
 }
 
-__device__ __forceinline__ unsigned nan_word(int type) {
-  return type == MFB200_TYPE_F32 ? 0x7FC00000u : type == MFB200_TYPE_BF16 ? 0x7FC07FC0u : 0x7E007E00u;
-}
-
-// Writes g[k] to the columns of the list, over the zeros that fill_row wrote.
-// A column that is listed more than once gets the sum of its values, in the
-// list's order. `seen`: one bit per column, shared memory of this warp.
-__device__ __forceinline__ void scatter_row(const Grad &out, const Moves &m, int classes, int b,
-                                            int lane, const float (&g)[kPerLane], unsigned *seen) {
-  const long long row = static_cast<long long>(b) * out.stride;
-  const int words = (classes + 31) >> 5;
-  for (int i = lane; i < words; i += 32) seen[i] = 0u;
-  __syncwarp();
-  bool again = false;
-  FOR_GROUPS(k, m.n) {
-    if (m.col[k] >= 0) {
-      const unsigned bit = 1u << (m.col[k] & 31);
-      again |= (atomicOr(seen + (m.col[k] >> 5), bit) & bit) != 0u;
+// Writes row b: g[k] at the columns of the list, 0 elsewhere. A column that is
+// listed more than once gets the sum of its values, in the list's order; the
+// moves find that out by leaving their numbers in the image.
+template <int G>
+__device__ __forceinline__ void write_row(RowImage &im, const Grad &out, int classes, int b, int n,
+                                          int lane, const int (&col)[G], float (&g)[G]) {
+  const int size = out.type == MFB200_TYPE_F32 ? 4 : 2;
+  char *dst = static_cast<char *>(out.base) + b * out.stride * size;
+  const int shift = static_cast<int>(reinterpret_cast<unsigned long long>(dst) & 127);
+  int at[G];
+  take_out(im, size, lane);
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+    at[k] = -1;
+    if (32 * k < n && col[k] >= 0) {
+      at[k] = shift + col[k] * size;
+      put(im.buf + at[k], size, 32 * k + lane + 1);
     }
   }
-  if (!__any_sync(kFull, again)) {
-    FOR_GROUPS(k, m.n) if (m.col[k] >= 0) store_as(out.base, out.type, row + m.col[k], g[k]);
-    return;
-  }
-  float sum[kPerLane];
-  bool first[kPerLane];
+  __syncwarp();
+  bool again = false;
 #pragma unroll
-  for (int k = 0; k < kPerLane; ++k) sum[k] = 0.0f, first[k] = true;
-  FOR_GROUPS(k2, m.n) {
-    for (int src = 0; src < 32 && 32 * k2 + src < m.n; ++src) {
-      const int c = __shfl_sync(kFull, m.col[k2], src);
-      const float v = __shfl_sync(kFull, g[k2], src);
-      FOR_GROUPS(k, m.n) {
-        if (m.col[k] == c) {
-          sum[k] += v;
-          if (32 * k2 + src < 32 * k + lane) first[k] = false;
+  for (int k = 0; k < G; ++k)
+    if (32 * k < n && at[k] >= 0) again |= get(im.buf + at[k], size) != 32u * k + lane + 1;
+  if (__any_sync(kFull, again)) {
+    float sum[G];
+    bool first[G];
+#pragma unroll
+    for (int k = 0; k < G; ++k) sum[k] = 0.0f, first[k] = true;
+#pragma unroll
+    for (int k2 = 0; k2 < G; ++k2) {
+      for (int src = 0; src < 32 && 32 * k2 + src < n; ++src) {
+        const int c = __shfl_sync(kFull, col[k2], src);
+        const float v = __shfl_sync(kFull, g[k2], src);
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+          if (col[k] == c) {
+            sum[k] += v;
+            if (32 * k2 + src < 32 * k + lane) first[k] = false;
+          }
         }
       }
     }
-  }
-  FOR_GROUPS(k, m.n)
-  if (m.col[k] >= 0 && first[k]) store_as(out.base, out.type, row + m.col[k], sum[k]);
-}
-
-__device__ __forceinline__ float quiet_nan() { return __int_as_float(0x7FC00000); }
-
-// ------------------------------------------------------------------ log-probabilities
-__global__ void __launch_bounds__(32 * kMaxWarps)
-    move_logprobs_kernel(PolicyRows r, float *move_logp,
-                         float *played_logp, float *entropy,
-                         float *row_state) {
-  pdl_wait();
-  pdl_launch();
-  const int lane = threadIdx.x & 31;
-  const unsigned at_row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (at_row >= static_cast<unsigned>(r.batch)) return;
-  const int b = static_cast<int>(at_row);
-  const Moves m = load_moves(r, load_head(r, b), lane);
-  float z[kPerLane], e[kPerLane];
-  load_logits(r, m, r.logits, r.stride, r.type, b, z);
-  const Norm q = normalise(m, z, r.inv_temp, lane, e);
-  float h = 0.0f;
-  FOR_GROUPS(k, m.n) {
-    const int j = 32 * k + lane;
-    if (j < m.n) {
-      const float logp = q.live ? (z[k] - q.top) * r.inv_temp - q.log_s : -INFINITY;
-      const float p = e[k] * q.inv_s;
-      if (p != 0.0f) h -= p * logp;  // 0 log 0 = 0; NaN passes
-      if (move_logp) move_logp[m.lo + j] = logp;
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      g[k] = sum[k];
+      if (!first[k]) at[k] = -1;
     }
   }
-  if (move_logp)
-    for (int j = m.n + lane; j < m.count; j += 32) move_logp[m.lo + j] = -INFINITY;
-  h = warp_sum(h);
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < G; ++k)
+    if (32 * k < n && at[k] >= 0) put(im.buf + at[k], size, bits_of(out.type, g[k]));
+  fence_proxy_async_smem();
+  __syncwarp();
+  // [shift, end) of the image is the row; [lo, hi) of it lies between 16-byte boundaries
+  const int end = shift + classes * size;
+  const int lo = (shift + 15) & ~15, hi = end & ~15;
+  if (lane == 0 && hi > lo) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst - shift + lo),
+                 "r"(smem_u32(im.buf + lo)), "r"(hi - lo)
+                 : "memory");
+    bulk_commit();
+  }
+  const int head = hi > lo ? (lo - shift) / size : classes;  // elements before the copy, and after
+  const int tail = hi > lo ? (end - hi) / size : 0;
+  if (lane < head + tail) {
+    const int p = lane < head ? shift + lane * size : hi + (lane - head) * size;
+    put(dst - shift + p, size, get(im.buf + p, size));
+  }
+  im.pending = true;
+  if (G == 2) {
+    im.old[0] = at[0];
+    im.old[1] = at[1];
+  } else {  // too many values to remember: take them out at once
+    if (lane == 0) bulk_wait_read0();
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+      if (32 * k < n && at[k] >= 0) put(im.buf + at[k], size, 0u);
+    __syncwarp();
+    im.pending = false;
+  }
+}
+
+// A row of NaN, for a malformed position.
+__device__ __forceinline__ void write_nan_row(const Grad &out, int classes, int b, int lane) {
+  const int size = out.type == MFB200_TYPE_F32 ? 4 : 2;
+  char *dst = static_cast<char *>(out.base) + b * out.stride * size;
+  for (int i = lane; i < classes; i += 32) put(dst + static_cast<long long>(i) * size, size, bits_of(out.type, quiet_nan()));
+}
+
+// ------------------------------------------------------------------ log-probabilities
+template <int G>
+__device__ __forceinline__ void score_position(const PolicyRows &r, float inv_temp2, int b,
+                                               const Moves &m, int c0, int c1, int lane,
+                                               float *move_logp, float *played_logp,
+                                               float *entropy, float *row_state) {
+  Edges<G> v;
+  columns<G>(r, m, c0, c1, lane, v);
+  load_logits<G>(m, row_of(r.logits, r.type, r.stride, b), r.type, v.col, v.z);
+  float es;
+  Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, inv_temp2, lane, v.e, es);
+  float none = 0.0f;
+  const float h = softmax_done<false>(q, es, q, none, lane);
+  if (move_logp) {
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      const int j = 32 * k + lane;
+      if (j < m.n)
+        move_logp[m.lo + j] = q.live ? (v.z[k] - q.top) * r.inv_temp - q.log_s : -INFINITY;
+    }
+    if (G > 2)
+      for (int j = m.n + lane; j < m.count; j += 32) move_logp[m.lo + j] = -INFINITY;
+  }
   const bool takes = q.live && m.played >= 0;
-  const float at = (of_move(z, m.n, m.played < 0 ? 0 : m.played) - q.top) * r.inv_temp - q.log_s;
+  const float z = of_move<G>(v.z, m.played < 0 ? 0 : m.played);
   if (lane == 0) {
-    if (played_logp) played_logp[b] = m.bad ? quiet_nan() : takes ? at : 0.0f;
+    if (played_logp)
+      played_logp[b] = m.bad ? quiet_nan() : takes ? (z - q.top) * r.inv_temp - q.log_s : 0.0f;
     if (entropy) entropy[b] = m.bad ? quiet_nan() : q.live ? h : 0.0f;
     if (row_state) row_state[b] = takes || m.bad ? 0.0f : -0.0f;
   }
 }
 
+__global__ void __launch_bounds__(32 * kMaxWarps)
+    move_logprobs_kernel(const __grid_constant__ PolicyRows r, float *move_logp, float *played_logp, float *entropy,
+                         float *row_state) {
+  __shared__ unsigned next_turn;
+  start_turns(&next_turn);
+  pdl_wait();
+  pdl_launch();
+  const int lane = threadIdx.x & 31;
+  const float inv_temp2 = r.inv_temp * kLog2e;
+  for_positions(
+      r, gridDim.x, &next_turn,
+      [&](int b, const Moves &m, int c0, int c1) {
+        if (m.n > 64) return true;
+        score_position<2>(r, inv_temp2, b, m, c0, c1, lane, move_logp, played_logp, entropy, row_state);
+        return false;
+      },
+      [&](int b, const Moves &m) {
+        score_position<8>(r, inv_temp2, b, m, load_index(r, m, 0, lane), load_index(r, m, 1, lane),
+                          lane, move_logp, played_logp, entropy, row_state);
+      });
+}
+
+// [c = a] - p_c for move j; 1 - p of the largest entry is rest / S
+__device__ __forceinline__ float played_term(const Moves &m, const Norm &q, int j, float p) {
+  return j != m.played ? -p : j == q.lead ? q.rest * q.inv_s : 1.0f - p;
+}
+
 // dL/dlogit_c = (1/T) [ G_c + [c = a] g - p_c (sum G + g) - g_H p_c (logp_c + H) ]
 // for upstream gradients G of the moves' log-probabilities, g of the played
 // move's and g_H of the entropy, each of which may be null.
-__global__ void __launch_bounds__(32 * kMaxWarps)
-    move_logprobs_backward_kernel(PolicyRows r, const float *grad_moves,
-                                  const float *grad_played,
-                                  const float *grad_entropy, Grad out) {
-  extern __shared__ unsigned seen_all[];
-  pdl_wait();
-  pdl_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned at_row = blockIdx.x * (blockDim.x >> 5) + warp;
-  if (at_row >= static_cast<unsigned>(r.batch)) return;
-  const int b = static_cast<int>(at_row);
-  const ListHead head = load_head(r, b);
-  fill_row(out, r.classes, b, lane, 0u);
-  const Moves m = load_moves(r, head, lane);
-  if (m.bad) {
-    __syncwarp();
-    fill_row(out, r.classes, b, lane, nan_word(out.type));
-    return;
-  }
-  float z[kPerLane], e[kPerLane], g[kPerLane];
-  load_logits(r, m, r.logits, r.stride, r.type, b, z);
-  float total = 0.0f;
-  FOR_GROUPS(k, m.n) {
-    const int j = 32 * k + lane;
-    g[k] = grad_moves && j < m.n ? grad_moves[m.lo + j] : 0.0f;
+struct BackArgs {
+  const float *moves, *played, *entropy;
+  Grad out;
+  // the sum of n losses, by one more CTA, where `total` is set
+  const float *loss;
+  int n;
+  float *total;
+};
+
+template <int G>
+__device__ __forceinline__ void back_position(const PolicyRows &r, const BackArgs &a,
+                                              float inv_temp2, int b, const Moves &m, int c0,
+                                              int c1, int lane, RowImage &im) {
+  Edges<G> v;
+  columns<G>(r, m, c0, c1, lane, v);
+  load_logits<G>(m, row_of(r.logits, r.type, r.stride, b), r.type, v.col, v.z);
+  float g[G], total = 0.0f;
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+    g[k] = a.moves && 32 * k + lane < m.n ? a.moves[m.lo + 32 * k + lane] : 0.0f;
     total += g[k];
   }
-  const float ga = grad_played && m.played >= 0 ? grad_played[b] : 0.0f;
-  const float gh = grad_entropy ? grad_entropy[b] : 0.0f;
-  const Norm q = normalise(m, z, r.inv_temp, lane, e);
-  if (!q.live) return;
-  total = warp_sum(total);
-  float h = 0.0f;
-  if (grad_entropy) {
-    FOR_GROUPS(k, m.n) {
-      const float p = e[k] * q.inv_s;
-      if (p != 0.0f) h -= p * ((z[k] - q.top) * r.inv_temp - q.log_s);
-    }
-    h = warp_sum(h);
-  }
-  FOR_GROUPS(k, m.n) {
+  const float ga = a.played && m.played >= 0 ? a.played[b] : 0.0f;
+  const float gh = a.entropy ? a.entropy[b] : 0.0f;
+  float es;
+  Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, inv_temp2, lane, v.e, es);
+  const float h = softmax_done<false>(q, es, q, total, lane);
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+    if (32 * k >= m.n) continue;
     const int j = 32 * k + lane;
-    const float p = e[k] * q.inv_s;
-    float v = g[k] - p * total;
-    // ([c = a] - p_c) g; 1 - p of the largest entry is rest / S
-    v += ga * (j != m.played ? -p : j == q.lead ? q.rest * q.inv_s : 1.0f - p);
-    if (grad_entropy && p != 0.0f)
-      v -= gh * p * ((z[k] - q.top) * r.inv_temp - q.log_s + h);
-    g[k] = v * r.inv_temp;
+    const float p = v.e[k] * q.inv_s;
+    float t = g[k] - p * total + ga * played_term(m, q, j, p);
+    if (a.entropy && p != 0.0f) t -= gh * p * ((v.z[k] - q.top) * r.inv_temp - q.log_s + h);
+    g[k] = t * r.inv_temp;
+    if (!q.live) v.col[k] = kNoColumn;
   }
-  scatter_row(out, m, r.classes, b, lane, g, seen_all + warp * ((r.classes + 31) >> 5));
+  write_row<G>(im, a.out, r.classes, b, m.n, lane, v.col, g);
+}
+
+// The sum of n losses by the `ctas` CTAs of a cluster (or one CTA), in 64 bits
+// and in one order.
+__device__ void sum_losses(const float *loss, int n, float *total, unsigned ctas) {
+  __shared__ double part[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned rank = ctas > 1 ? blockIdx.x : 0;
+  double v = 0.0;
+  const long long step = static_cast<long long>(blockDim.x) * ctas;
+  long long i = static_cast<long long>(rank) * blockDim.x + threadIdx.x;
+  for (; n - i > 15 * step; i += 16 * step) {  // sixteen loads under way at once
+    float x[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) x[k] = loss[i + k * step];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v += x[k];
+  }
+  float x[15];
+#pragma unroll
+  for (int k = 0; k < 15; ++k) x[k] = i + k * step < n ? loss[i + k * step] : 0.0f;
+#pragma unroll
+  for (int k = 0; k < 15; ++k) v += x[k];
+  v = warp_sum(v);
+  if (lane == 0) part[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    v = lane < static_cast<int>(blockDim.x >> 5) ? part[lane] : 0.0;
+    v = warp_sum(v);
+    if (ctas == 1) {
+      if (lane == 0) *total = static_cast<float>(v);
+      return;
+    }
+    if (lane == 0) part[0] = v;
+  }
+  if (ctas == 1) return;
+  cluster_sync();
+  if (rank == 0 && warp == 0) {
+    double w = 0.0;
+    if (lane < static_cast<int>(ctas)) {
+      unsigned at;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(part)), "r"(lane));
+      asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(w) : "r"(at));
+    }
+    w = warp_sum(w);
+    if (lane == 0) *total = static_cast<float>(w);
+  }
+  cluster_sync();  // no CTA leaves while its part is read
+}
+
+__global__ void __launch_bounds__(32 * kMaxWarps, 3)
+    move_logprobs_backward_kernel(const __grid_constant__ PolicyRows r,
+                                  const __grid_constant__ BackArgs a) {
+  extern __shared__ __align__(128) char images[];
+  const int lane = threadIdx.x & 31;
+  const int row_bytes = r.classes * (a.out.type == MFB200_TYPE_F32 ? 4 : 2);
+  const unsigned ctas = gridDim.x - (a.total ? 1 : 0);
+  RowImage im = clear_image(images + (threadIdx.x >> 5) * image_bytes(row_bytes), row_bytes, lane);
+  __shared__ unsigned next_turn;
+  start_turns(&next_turn);
+  pdl_wait();
+  pdl_launch();
+  if (blockIdx.x == ctas) {
+    sum_losses(a.loss, a.n, a.total, 1);
+    return;
+  }
+  const float inv_temp2 = r.inv_temp * kLog2e;
+  for_positions(
+      r, ctas, &next_turn,
+      [&](int b, const Moves &m, int c0, int c1) {
+        if (m.n > 64 || m.bad) return true;
+        back_position<2>(r, a, inv_temp2, b, m, c0, c1, lane, im);
+        return false;
+      },
+      [&](int b, const Moves &m) {
+        if (m.bad)
+          write_nan_row(a.out, r.classes, b, lane);
+        else
+          back_position<8>(r, a, inv_temp2, b, m, load_index(r, m, 0, lane),
+                           load_index(r, m, 1, lane), lane, im);
+      });
+  if (lane == 0) bulk_wait0();
 }
 
 // ------------------------------------------------------------------ clipped policy loss
@@ -365,103 +680,141 @@ struct ClipArgs {
   Grad grad;
 };
 
-// e^-d - 1 + d, the contribution of a move to KL = sum p (e^-d - 1 + d) with
-// d = log p - log q (sum p e^-d = sum q = 1). Every term is >= 0 and an error
-// common to all d cancels, so the KL of two near policies keeps its digits.
-// Taylor series for |d| < 1, where the exponential would cancel.
-__device__ __forceinline__ float kl_term(float d) {
-  float t = 1.0f;
-#pragma unroll
-  for (int i = 13; i >= 3; --i) t = 1.0f - d * (1.0f / i) * t;
-  return 0.5f * d * d * t;
+// KL = sum p (e^-d - 1 + d) with d = log p - log q (sum p e^-d = sum q = 1):
+// every term is >= 0 and an error common to all d cancels, so the KL of two
+// near policies keeps its digits. For |d| < 1/2 by the series d^2/2 - d^3/6 +
+// ... + d^8/8!, whose next term is 3e-8 of it; else from p, q and d themselves.
+__device__ __forceinline__ float kl_term(float p, float pr, float d) {
+  float t = 1.0f / 40320;
+  t = fmaf(t, -d, 1.0f / 5040);
+  t = fmaf(t, -d, 1.0f / 720);
+  t = fmaf(t, -d, 1.0f / 120);
+  t = fmaf(t, -d, 1.0f / 24);
+  t = fmaf(t, -d, 1.0f / 6);
+  t = fmaf(t, -d, 1.0f / 2);
+  const float near = p * (d * d * t), far = pr - p + p * d;
+  return p == 0.0f ? pr : fabsf(d) < 0.5f ? near : far;
 }
 
-__global__ void __launch_bounds__(32 * kMaxWarps)
-    clipped_policy_loss_kernel(PolicyRows r, ClipArgs a) {
-  extern __shared__ unsigned seen_all[];
-  pdl_wait();
-  pdl_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned at_row = blockIdx.x * (blockDim.x >> 5) + warp;
-  if (at_row >= static_cast<unsigned>(r.batch)) return;
-  const int b = static_cast<int>(at_row);
-  const ListHead head = load_head(r, b);
+// Returns true, with nothing written, for a ratio too near the clip's border
+// to be decided in 32 bits, unless kExact.
+template <int G, bool kExact>
+__device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArgs &a,
+                                              float inv_temp2, int b, const Moves &m, int c0,
+                                              int c1, int lane, RowImage &im) {
+  Edges<G> v;
+  columns<G>(r, m, c0, c1, lane, v);
+  const void *row = row_of(r.logits, r.type, r.stride, b);
+  load_logits<G>(m, row, r.type, v.col, v.z);
+  float d[G];  // the reference's logits, then d = log p - log q
+  if (a.ref) load_logits<G>(m, row_of(a.ref, a.ref_type, a.ref_stride, b), a.ref_type, v.col, d);
   const float old = a.old_logp[b], adv = a.advantage[b];
-  const float c0 = a.scale * (a.weight ? a.weight[b] : 1.0f);
-  if (a.grad.base) fill_row(a.grad, r.classes, b, lane, 0u);
-  const Moves m = load_moves(r, head, lane);
-  float z[kPerLane], e[kPerLane], zr[kPerLane], d[kPerLane];
-  load_logits(r, m, r.logits, r.stride, r.type, b, z);
-  if (a.ref) load_logits(r, m, a.ref, a.ref_stride, a.ref_type, b, zr);
-  const Norm q = normalise(m, z, r.inv_temp, lane, e);
-  const bool takes = q.live && m.played >= 0;
-
-  float h = 0.0f;
-  FOR_GROUPS(k, m.n) {
-    const float p = e[k] * q.inv_s;
-    if (p != 0.0f) h -= p * ((z[k] - q.top) * r.inv_temp - q.log_s);
-  }
-  h = q.live ? warp_sum(h) : 0.0f;
-  float kl = 0.0f;
+  const float c = a.scale * (a.weight ? a.weight[b] : 1.0f);
+  float es;
+  Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, inv_temp2, lane, v.e, es);
+  float h, kl = 0.0f;
   if (a.ref) {
-    const Norm w = normalise(m, zr, r.inv_temp, lane, d);  // d: exp(s - s_top) of the reference
-    FOR_GROUPS(k, m.n) {
-      const float p = e[k] * q.inv_s, pr = d[k] * w.inv_s;
-      // d = log p - log q: the near logits are subtracted first
-      d[k] = ((z[k] - zr[k]) - (q.top - w.top)) * r.inv_temp + (w.log_s - q.log_s);
-      if (32 * k + lane < m.n)
-        kl += p == 0.0f ? pr : fabsf(d[k]) < 1.0f ? p * kl_term(d[k]) : pr - p + p * d[k];
+    float er[G], es_r;
+    Norm w = softmax_part<G>(m.n, d, r.inv_temp, inv_temp2, lane, er, es_r);
+    h = softmax_done<true>(q, es, w, kl, lane);
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      if (32 * k < m.n) {
+        // the near logits are subtracted first
+        d[k] = ((v.z[k] - d[k]) - (q.top - w.top)) * r.inv_temp + (w.log_s - q.log_s);
+        kl += kl_term(v.e[k] * q.inv_s, er[k] * w.inv_s, d[k]);
+      }
     }
-    kl = q.live ? warp_sum(kl) : 0.0f;
+    kl = warp_sum(kl);
+  } else {
+    h = softmax_done<false>(q, es, q, kl, lane);
   }
-
-  const float sa = (of_move(z, m.n, m.played < 0 ? 0 : m.played) - q.top) * r.inv_temp;
-  const float ratio = expf((sa - old) - q.log_s);
+  const bool takes = q.live && m.played >= 0;
+  const float za = of_move<G>(v.z, m.played < 0 ? 0 : m.played);
+  const float sa = (za - q.top) * r.inv_temp;
+  const float ratio = exp2_fast(((sa - old) - q.log_s) * kLog2e);
   // The gradient jumps where the ratio crosses the clip's border, so a ratio
   // within the rounding of the border is computed again in 64 bits.
   const float border = static_cast<float>(adv > 0.0f ? a.high : a.low);
   bool active = adv > 0.0f ? !(ratio > border) : !(ratio < border);
-  if (takes && fabsf(ratio - border) <= border * (2e-6f + 1e-6f * (fabsf(sa) + q.log_s + fabsf(old)))) {
+  if (takes && fabsf(ratio - border) <=
+                   border * (4e-6f + 1e-6f * (fabsf(sa) + q.log_s + fabsf(old)))) {
+    if (!kExact) return true;
     double sum = 0.0;
-    FOR_GROUPS(k, m.n)
-    if (32 * k + lane < m.n)
-      sum += exp((static_cast<double>(z[k]) - q.top) / r.temp);
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+      if (32 * k < m.n) sum += exp((static_cast<double>(v.z[k]) - q.top) / r.temp);
     sum = warp_sum(sum);
-    const double za = of_move(z, m.n, m.played);
-    const double exact = exp((za - q.top) / r.temp - log(sum) - static_cast<double>(old));
+    const double exact =
+        exp((static_cast<double>(za) - q.top) / r.temp - log(sum) - static_cast<double>(old));
     active = adv > 0.0f ? !(exact > a.high) : !(exact < a.low);
   }
+  if (a.grad.base) {
+    const float slope = active ? -adv * ratio : 0.0f;
+    float g[G];
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      if (32 * k >= m.n) continue;
+      const float p = v.e[k] * q.inv_s;
+      float t = slope * played_term(m, q, 32 * k + lane, p);
+      if (p != 0.0f) {
+        if (a.ref) t += a.kl_coef * p * (d[k] - kl);
+        t += a.entropy_coef * p * ((v.z[k] - q.top) * r.inv_temp - q.log_s + h);
+      }
+      g[k] = c * r.inv_temp * t;
+      if (!takes) v.col[k] = kNoColumn;
+    }
+    write_row<G>(im, a.grad, r.classes, b, m.n, lane, v.col, g);
+  }
+  // after the row: the fence before its copy would wait for these stores
   if (lane == 0) {
-    const float bad = quiet_nan();
     float loss = -adv * (active ? ratio : border);
     if (a.ref) loss += a.kl_coef * kl;
     loss -= a.entropy_coef * h;
-    if (a.loss) a.loss[b] = m.bad ? bad : takes ? c0 * loss : 0.0f;
-    if (a.logp) a.logp[b] = m.bad ? bad : takes ? sa - q.log_s : 0.0f;
-    if (a.kl) a.kl[b] = m.bad ? bad : kl;
-    if (a.entropy) a.entropy[b] = m.bad ? bad : h;
+    if (a.loss) a.loss[b] = takes ? c * loss : 0.0f;
+    if (a.logp) a.logp[b] = takes ? sa - q.log_s : 0.0f;
+    if (a.kl) a.kl[b] = q.live ? kl : 0.0f;
+    if (a.entropy) a.entropy[b] = q.live ? h : 0.0f;
   }
-  if (!a.grad.base) return;
-  if (m.bad) {
-    __syncwarp();
-    fill_row(a.grad, r.classes, b, lane, nan_word(a.grad.type));
-    return;
+  return false;
+}
+
+__global__ void __launch_bounds__(32 * kMaxWarps, 3)
+    clipped_policy_loss_kernel(const __grid_constant__ PolicyRows r,
+                               const __grid_constant__ ClipArgs a) {
+  extern __shared__ __align__(128) char images[];
+  const int lane = threadIdx.x & 31;
+  RowImage im{};
+  if (a.grad.base) {
+    const int row_bytes = r.classes * (a.grad.type == MFB200_TYPE_F32 ? 4 : 2);
+    im = clear_image(images + (threadIdx.x >> 5) * image_bytes(row_bytes), row_bytes, lane);
   }
-  if (!takes) return;
-  const float c = c0 * r.inv_temp;
-  const float slope = active ? -adv * ratio : 0.0f;
-  float g[kPerLane];
-  FOR_GROUPS(k, m.n) {
-    const int j = 32 * k + lane;
-    const float p = e[k] * q.inv_s;
-    float v = slope * (j != m.played ? -p : j == q.lead ? q.rest * q.inv_s : 1.0f - p);
-    if (p != 0.0f) {
-      if (a.ref) v += a.kl_coef * p * (d[k] - kl);
-      v += a.entropy_coef * p * ((z[k] - q.top) * r.inv_temp - q.log_s + h);
-    }
-    g[k] = c * v;
-  }
-  scatter_row(a.grad, m, r.classes, b, lane, g, seen_all + warp * ((r.classes + 31) >> 5));
+  __shared__ unsigned next_turn;
+  start_turns(&next_turn);
+  pdl_wait();
+  pdl_launch();
+  const float inv_temp2 = r.inv_temp * kLog2e;
+  for_positions(
+      r, gridDim.x, &next_turn,
+      [&](int b, const Moves &m, int c0, int c1) {
+        if (m.n > 64 || m.bad) return true;
+        return clip_position<2, false>(r, a, inv_temp2, b, m, c0, c1, lane, im);
+      },
+      [&](int b, const Moves &m) {
+        if (!m.bad) {
+          clip_position<8, true>(r, a, inv_temp2, b, m, load_index(r, m, 0, lane),
+                                 load_index(r, m, 1, lane), lane, im);
+          return;
+        }
+        if (lane == 0) {
+          if (a.loss) a.loss[b] = quiet_nan();
+          if (a.logp) a.logp[b] = quiet_nan();
+          if (a.kl) a.kl[b] = quiet_nan();
+          if (a.entropy) a.entropy[b] = quiet_nan();
+        }
+        if (a.grad.base) write_nan_row(a.grad, r.classes, b, lane);
+      });
+  if (lane == 0) bulk_wait0();
 }
 
 // ------------------------------------------------------------------ preference loss
@@ -524,57 +877,94 @@ __global__ void __launch_bounds__(256)
 }
 
 // ------------------------------------------------------------------ total
-// The sum of the losses, in 64 bits and in one order.
-__global__ void __launch_bounds__(1024)
-    loss_total_kernel(const float *loss, int n, float *total) {
-  __shared__ double part[32];
+__global__ void __launch_bounds__(1024) loss_total_kernel(const float *loss, int n, float *total) {
   pdl_wait();
   pdl_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  double v = 0.0;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) v += loss[i];
-  v = warp_sum(v);
-  if (lane == 0) part[warp] = v;
-  __syncthreads();
-  if (warp == 0) {
-    v = lane < static_cast<int>(blockDim.x >> 5) ? part[lane] : 0.0;
-    v = warp_sum(v);
-    if (lane == 0) *total = static_cast<float>(v);
-  }
+  sum_losses(loss, n, total, gridDim.x);
 }
 
 // ------------------------------------------------------------------ launches
-// Warps (positions) per CTA: one while the positions fit one per SM, so that
-// each has an SM's load units to itself, up to eight.
-int warps_for(int batch) {
+struct Shape {
+  int warps, ctas;
+  size_t smem;
+};
+
+// Positions are spread over the SMs before they share a CTA; a CTA's warps
+// then take `per_sm` CTAs' worth of positions in turn.
+Shape shape_for(int batch, int max_warps, int per_sm, size_t bytes_per_warp) {
+  const int sms = num_sms();
   int w = 1;
-  while (w < kMaxWarps && batch > 148 * w) w *= 2;
-  return w;
+  while (w < max_warps && batch > sms * w) w *= 2;
+  const long long need = (static_cast<long long>(batch) + w - 1) / w;
+  const long long most = static_cast<long long>(sms) * per_sm;
+  return {w, static_cast<int>(need < most ? need : most), w * bytes_per_warp};
 }
 
-size_t seen_bytes(const PolicyRows &r, int warps) {
-  return static_cast<size_t>(warps) * ((r.classes + 31) / 32) * sizeof(unsigned);
+// With a row image per warp: as many warps as keep three CTAs on an SM.
+Shape shape_with_images(const PolicyRows &r, const Grad &g) {
+  constexpr size_t kPerSm = 225 * 1024, kReserved = 1024;
+  const size_t bytes =
+      (static_cast<size_t>(r.classes) * (g.type == MFB200_TYPE_F32 ? 4 : 2) + 127) / 128 * 128 + 128;
+  int w = kMaxWarps;
+  while (w > 1 && 3 * (w * bytes + kReserved) > kPerSm) w /= 2;
+  const Shape s = shape_for(r.batch, w, 1, bytes);
+  int per_sm = static_cast<int>(kPerSm / (s.smem + kReserved));
+  per_sm = per_sm > 3 ? 3 : per_sm < 1 ? 1 : per_sm;
+  return shape_for(r.batch, w, per_sm, bytes);
 }
 
-cudaError_t launch_backward(const PolicyRows &r, const float *grad_moves, const float *grad_played,
-                            const float *grad_entropy, const Grad &g, cudaStream_t s) {
-  const int w = warps_for(r.batch);
-  return launch_k(move_logprobs_backward_kernel, dim3((r.batch + w - 1) / w), dim3(32 * w),
-                  seen_bytes(r, w), s, 1, r, grad_moves, grad_played, grad_entropy, g);
+// Raises a kernel's shared-memory limit once per device to what the largest row needs.
+template <class K>
+cudaError_t allow_images(K *kernel, std::atomic<unsigned long long> &done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  if (e == cudaSuccess) done.fetch_or(bit);
+  return e;
+}
+
+cudaError_t launch_backward(const PolicyRows &r, const BackArgs &a, cudaStream_t s) {
+  static std::atomic<unsigned long long> done{0};
+  if (cudaError_t e = allow_images(move_logprobs_backward_kernel, done)) return e;
+  const Shape t = shape_with_images(r, a.out);
+  return launch_k(move_logprobs_backward_kernel, dim3(t.ctas + (a.total ? 1 : 0)),
+                  dim3(32 * t.warps), t.smem, s, 1, r, a);
+}
+
+cudaError_t launch_clip(const PolicyRows &r, const ClipArgs &a, cudaStream_t s) {
+  static std::atomic<unsigned long long> done{0};
+  if (cudaError_t e = allow_images(clipped_policy_loss_kernel, done)) return e;
+  const Shape t = a.grad.base ? shape_with_images(r, a.grad) : shape_for(r.batch, kMaxWarps, 3, 0);
+  return launch_k(clipped_policy_loss_kernel, dim3(t.ctas), dim3(32 * t.warps), t.smem, s, 1, r, a);
+}
+
+cudaError_t launch_pairs(int pairs, int batch, const int32_t *lines, const float *logp,
+                         const float *ref, const float *weight, float beta, float eps, float scale,
+                         float *row_grad, float *line_logp, float *margin, float *loss,
+                         cudaStream_t s) {
+  int w = 1;
+  while (w < 8 && pairs > num_sms() * w) w *= 2;
+  return launch_k(preference_pair_kernel, dim3((static_cast<unsigned>(pairs) + w - 1) / w),
+                  dim3(32 * w), 0, s, 1, pairs, batch, lines, logp, ref, weight, beta, eps, scale,
+                  row_grad, line_logp, margin, loss);
 }
 
 cudaError_t launch_total(const float *loss, int n, float *total, cudaStream_t s) {
-  const int threads = n >= 1024 ? 1024 : (n + 31) / 32 * 32;
-  return launch_k(loss_total_kernel, dim3(1), dim3(threads ? threads : 32), 0, s, 1, loss, n, total);
+  const int threads = n >= 1024 ? 1024 : n > 0 ? (n + 31) / 32 * 32 : 32;
+  const int ctas = n > 16384 ? 8 : 1;  // more than 16 losses a thread: a cluster
+  return launch_k(loss_total_kernel, dim3(ctas), dim3(threads), 0, s, ctas, loss, n, total);
 }
 
 }  // namespace
 
 cudaError_t launch_move_logprobs(const PolicyRows &r, float *move_logp, float *played_logp,
                                  float *entropy, float *row_state, cudaStream_t s) {
-  const int w = warps_for(r.batch);
-  return launch_k(move_logprobs_kernel, dim3((r.batch + w - 1) / w), dim3(32 * w), 0, s, 1, r,
-                  move_logp, played_logp, entropy, row_state);
+  const Shape t = shape_for(r.batch, kMaxWarps, 6, 0);
+  return launch_k(move_logprobs_kernel, dim3(t.ctas), dim3(32 * t.warps), 0, s, 1, r, move_logp,
+                  played_logp, entropy, row_state);
 }
 
 }  // namespace mfb200
@@ -724,9 +1114,12 @@ extern "C" MFB200_API int mfb200_move_logprobs_backward(
       g.meets(array(rows->move_index, rows->num_moves, 2)) || g.meets(array(rows->played, n, 4)))
     return fail(fn, "the gradient overlaps an input");
   if (const char *e = check_device(rows->logits)) return fail(fn, e);
-  return launched(fn, launch_backward(rows_of(*rows), d_grad_moves, d_grad_played, d_grad_entropy,
-                                      Grad{d_grad_logits, grad_stride, grad_type},
-                                      static_cast<cudaStream_t>(stream)));
+  BackArgs a{};
+  a.moves = d_grad_moves;
+  a.played = d_grad_played;
+  a.entropy = d_grad_entropy;
+  a.out = Grad{d_grad_logits, grad_stride, grad_type};
+  return launched(fn, launch_backward(rows_of(*rows), a, static_cast<cudaStream_t>(stream)));
 }
 
 extern "C" MFB200_API int mfb200_clipped_policy_loss(
@@ -786,10 +1179,7 @@ extern "C" MFB200_API int mfb200_clipped_policy_loss(
   a.kl = d_kl;
   a.entropy = d_entropy;
   a.grad = Grad{d_grad_logits, grad_stride, grad_type};
-  const PolicyRows r = rows_of(*rows);
-  const int w = warps_for(n);
-  const cudaError_t e = launch_k(clipped_policy_loss_kernel, dim3((n + w - 1) / w), dim3(32 * w),
-                                 seen_bytes(r, w), s, 1, r, a);
+  const cudaError_t e = launch_clip(rows_of(*rows), a, s);
   if (e != cudaSuccess || !d_total) return launched(fn, e);
   return launched(fn, launch_total(d_loss, n, d_total, s));
 }
@@ -841,19 +1231,26 @@ extern "C" MFB200_API int mfb200_preference_loss(
   const PolicyRows r = rows_of(*rows);
   cudaError_t e = cudaSuccess;
   if (n > 0) e = launch_move_logprobs(r, nullptr, d_logp, nullptr, d_row_grad, s);
-  if (e == cudaSuccess && pairs > 0) {
-    const int w = warps_for(pairs);
-    e = launch_k(preference_pair_kernel, dim3((pairs + w - 1) / w), dim3(32 * w), 0, s, 1, pairs, n,
-                 d_line_offsets, static_cast<const float *>(d_logp), d_ref_logp, d_weight, cfg->beta,
-                 cfg->label_smoothing, cfg->scale, d_row_grad, d_line_logp, d_margin, d_loss);
+  if (e == cudaSuccess && pairs > 0)
+    e = launch_pairs(pairs, n, d_line_offsets, d_logp, d_ref_logp, d_weight, cfg->beta,
+                     cfg->label_smoothing, cfg->scale, d_row_grad, d_line_logp, d_margin, d_loss, s);
+  const bool with_grad = n > 0 && d_grad_logits;
+  if (e == cudaSuccess && with_grad) {
+    BackArgs a{};
+    a.played = d_row_grad;
+    a.out = Grad{d_grad_logits, grad_stride, grad_type};
+    if (pairs > 0 && d_total) {
+      a.loss = d_loss;
+      a.n = pairs;
+      a.total = d_total;
+    }
+    e = launch_backward(r, a, s);
   }
-  if (e == cudaSuccess && n > 0 && d_grad_logits)
-    e = launch_backward(r, nullptr, d_row_grad, nullptr, Grad{d_grad_logits, grad_stride, grad_type}, s);
   if (e == cudaSuccess && d_total) {
-    if (pairs > 0)
-      e = launch_total(d_loss, pairs, d_total, s);
-    else
+    if (pairs == 0)
       e = cudaMemsetAsync(d_total, 0, sizeof(float), s);
+    else if (!with_grad)
+      e = launch_total(d_loss, pairs, d_total, s);
   }
   return launched(fn, e);
 }
