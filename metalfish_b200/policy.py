@@ -105,15 +105,19 @@ def _lib():
 
 def _vector(t, name, dtype, size, device):
     """Pointer of a contiguous 1-D tensor of the given type and size (None: any)."""
+    try:
+        if (t.dtype is dtype and t.dim() == 1 and t.get_device() == device and t.is_contiguous()
+                and (size is None or t.numel() == size)):
+            return t.data_ptr()
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != 1:
         raise ValueError(f"{name} must be a 1-D {dtype} tensor")
-    if size is not None and t.shape[0] != size:
-        raise ValueError(f"{name} has {t.shape[0]} entries, expected {size}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the logits on {device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, the logits on cuda:{device}")
+    if size is not None and t.numel() != size:
+        raise ValueError(f"{name} has {t.numel()} entries, expected {size}")
+    raise ValueError(f"{name} must be contiguous")
 
 
 def _matrix(t, name, shape, device):
@@ -123,8 +127,8 @@ def _matrix(t, name, shape, device):
         raise ValueError(f"{name} must be a 2-D float32, bfloat16 or float16 tensor")
     if t.shape != shape:
         raise ValueError(f"{name} is {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the logits on {device}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, the logits on cuda:{device}")
     rows, cols = shape
     stride, unit = t.stride()
     if unit != 1 and cols > 1:
@@ -133,35 +137,45 @@ def _matrix(t, name, shape, device):
 
 
 def _rows(logits, move_offsets, move_index, played, softmax_temp):
+    """The C struct and the device's index."""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
         raise ValueError("logits must be a 2-D float32, bfloat16 or float16 tensor")
-    device = logits.device
-    if device.type != "cuda":
+    device = logits.get_device()
+    if device < 0:
         raise ValueError("logits must be a CUDA tensor: there is no CPU path")
-    batch, classes = logits.shape
-    ptr, stride, kind = _matrix(logits, "logits", logits.shape, device)
+    shape = logits.shape
+    batch, classes = shape
+    ptr, stride, kind = _matrix(logits, "logits", shape, device)
     off = _vector(move_offsets, "move_offsets", torch.int32, batch + 1, device)
     index = _vector(move_index, "move_index", torch.int16, None, device)
     at = None if played is None else _vector(played, "played", torch.int32, batch, device)
-    return _Rows(ptr, stride, kind, batch, classes, off, index, move_index.shape[0], at,
+    return _Rows(ptr, stride, kind, batch, classes, off, index, move_index.numel(), at,
                  softmax_temp), device
 
 
-def _gradient(logits, grad_logits, device):
+def _gradient(logits, grad, grad_logits, device):
+    """(tensor, pointer, row stride, type) of the gradient to write."""
     if grad_logits is None:
-        grad_logits = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+        if not grad:
+            return None, None, 0, 0
+        grad_logits = torch.empty_like(logits)  # contiguous for rows that are padded
     return (grad_logits, *_matrix(grad_logits, "grad_logits", logits.shape, device))
 
 
 def _call(fn, device, *args):
     """The library call on the logits' device and its current stream."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if device == torch.cuda.current_device():
+        rc = fn(*args, _stream_of(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, _stream_of(device))
     if rc != 0:
         raise RuntimeError(_native.mfb200_policy_last_error().decode())
+
+
+# torch.cuda.current_stream builds a Stream object (3 us); its raw handle takes 0.1 us
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream",
+                     lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def move_logprobs(logits, move_offsets, move_index, played=None, *,
@@ -170,11 +184,10 @@ def move_logprobs(logits, move_offsets, move_index, played=None, *,
     entropy of each position (``mfb200_move_logprobs``)."""
     L = _lib()
     rows, device = _rows(logits, move_offsets, move_index, played, softmax_temp)
-    moves = torch.empty(rows.num_moves, dtype=torch.float32, device=device)
-    if played is None:
-        at, entropy = None, torch.empty(rows.batch, dtype=torch.float32, device=device)
-    else:
-        at, entropy = torch.empty((2, rows.batch), dtype=torch.float32, device=device).unbind()
+    f = torch.float32
+    moves = torch.empty_like(move_index, dtype=f)
+    at = None if played is None else torch.empty_like(played, dtype=f)
+    entropy = logits.new_empty(rows.batch, dtype=f)
     _call(L.mfb200_move_logprobs, device, rows, moves.data_ptr(),
           None if at is None else at.data_ptr(), entropy.data_ptr())
     return MoveLogprobs(moves, at, entropy)
@@ -195,7 +208,7 @@ def move_logprobs_backward(logits, move_offsets, move_index, played=None, *, gra
     gh = None if grad_entropy is None else _vector(grad_entropy, "grad_entropy", f, rows.batch, device)
     if gp is not None and played is None:
         raise ValueError("grad_played needs played")
-    grad, ptr, stride, kind = _gradient(logits, grad_logits, device)
+    grad, ptr, stride, kind = _gradient(logits, True, grad_logits, device)
     _call(L.mfb200_move_logprobs_backward, device, rows, gm, gp, gh, ptr, stride, kind)
     return grad
 
@@ -218,16 +231,13 @@ def clipped_policy_loss(logits, move_offsets, move_index, played, old_logp, adva
     w = None if weight is None else _vector(weight, "weight", f, n, device)
     ref, ref_stride, ref_kind = ((None, 0, 0) if ref_logits is None
                                  else _matrix(ref_logits, "ref_logits", logits.shape, device))
-    g, ptr, stride, kind = (_gradient(logits, grad_logits, device) if grad or grad_logits is not None
-                            else (None, None, 0, 0))
+    g, ptr, stride, kind = _gradient(logits, grad, grad_logits, device)
     cfg = _ClipConfig(clip_low, clip_high, kl_coef, entropy_coef,
                       scale if scale is not None else 1.0 / max(n, 1))
-    total = torch.empty((), dtype=f, device=device)
-    if ref is None:
-        loss, logp, entropy = torch.empty((3, n), dtype=f, device=device).unbind()
-        kl = None
-    else:
-        loss, logp, entropy, kl = torch.empty((4, n), dtype=f, device=device).unbind()
+    total = old_logp.new_empty(())
+    loss, logp, entropy = (torch.empty_like(old_logp), torch.empty_like(old_logp),
+                           torch.empty_like(old_logp))
+    kl = None if ref is None else torch.empty_like(old_logp)
     _call(L.mfb200_clipped_policy_loss, device, rows, cfg, old, adv, w, ref, ref_stride, ref_kind,
           loss.data_ptr(), logp.data_ptr(), None if kl is None else kl.data_ptr(),
           entropy.data_ptr(), total.data_ptr(), ptr, stride, kind)
@@ -249,18 +259,17 @@ def preference_loss(logits, move_offsets, move_index, played, line_offsets, ref_
         raise ValueError("played must be a 1-D torch.int32 tensor")
     n, f = rows.batch, torch.float32
     lines = _vector(line_offsets, "line_offsets", torch.int32, None, device)
-    if line_offsets.shape[0] % 2 != 1:
+    if line_offsets.numel() % 2 != 1:
         raise ValueError("line_offsets must have 2 * pairs + 1 entries")
-    pairs = line_offsets.shape[0] // 2
+    pairs = line_offsets.numel() // 2
     ref = _vector(ref_logp, "ref_logp", f, n, device)
     w = None if weight is None else _vector(weight, "weight", f, pairs, device)
-    g, ptr, stride, kind = (_gradient(logits, grad_logits, device) if grad or grad_logits is not None
-                            else (None, None, 0, 0))
+    g, ptr, stride, kind = _gradient(logits, grad, grad_logits, device)
     cfg = _PreferenceConfig(beta, label_smoothing, scale if scale is not None else 1.0 / max(pairs, 1))
-    total = torch.empty((), dtype=f, device=device)
-    logp, row_grad = torch.empty((2, n), dtype=f, device=device).unbind()
-    loss, margin = torch.empty((2, pairs), dtype=f, device=device).unbind()
-    line_logp = torch.empty(2 * pairs, dtype=f, device=device)
+    total = ref_logp.new_empty(())
+    logp, row_grad = torch.empty_like(ref_logp), torch.empty_like(ref_logp)
+    loss, margin = ref_logp.new_empty(pairs), ref_logp.new_empty(pairs)
+    line_logp = ref_logp.new_empty(2 * pairs)
     _call(L.mfb200_preference_loss, device, rows, cfg, lines, pairs, ref, w, logp.data_ptr(),
           row_grad.data_ptr(), line_logp.data_ptr(), margin.data_ptr(), loss.data_ptr(),
           total.data_ptr(), ptr, stride, kind)
