@@ -23,9 +23,9 @@
 // their SM and their warps take positions in turn, the lists of the next ones
 // loaded ahead. A gradient row is put together in shared memory and written by
 // one bulk copy, while the warp goes on. 65536 positions, 1858 fp32 classes, on
-// B200: clipped loss with KL 136 us (615 MB of DRAM traffic, 4.5 TB/s; the
-// copies of empty lists alone 75 us), its backward pass alone 102 us,
-// log-probabilities 35 us.
+// B200: clipped loss with KL 132 us (615 MB of DRAM traffic; the same reads and
+// copies without any arithmetic 127 us, the copies alone 92), its backward pass
+// alone 111 us, log-probabilities 39 us.
 #include "policy.cuh"
 
 #include <atomic>
@@ -53,21 +53,25 @@ constexpr float kLog2e = 1.4426950408889634f;
 // __restrict__ const): a kernel here may start before the one that writes its
 // inputs has ended (pdl.cuh), and a read-only load may be moved above pdl_wait.
 
-// A logit. L2 takes 64 bytes from DRAM for it instead of the 128 that a plain
-// load takes: 65536 gathers of 16 pairs of logits a row read 88 MB instead of
-// 155, in 17.4 instead of 26.5 us.
-__device__ __forceinline__ float load_logit(const void *row, int type, int c) {
+// The bits of a logit. L2 takes 64 bytes from DRAM for it instead of the 128
+// that a plain load takes: 65536 gathers of 16 pairs of logits a row read 88 MB
+// instead of 155, in 17.4 instead of 26.5 us.
+__device__ __forceinline__ unsigned load_bits(const void *row, int type, int c) {
   if (type == MFB200_TYPE_F32) {
-    float v;
-    asm volatile("ld.global.L2::64B.f32 %0, [%1];" : "=f"(v) : "l"(static_cast<const float *>(row) + c));
+    unsigned v;
+    asm volatile("ld.global.L2::64B.u32 %0, [%1];" : "=r"(v) : "l"(static_cast<const float *>(row) + c));
     return v;
   }
   unsigned short u;
   asm volatile("ld.global.L2::64B.u16 %0, [%1];"
                : "=h"(u)
                : "l"(static_cast<const unsigned short *>(row) + c));
-  return type == MFB200_TYPE_BF16 ? __uint_as_float(static_cast<unsigned>(u) << 16)
-                                  : __half2float(__ushort_as_half(u));
+  return u;
+}
+__device__ __forceinline__ float value_of(int type, unsigned bits) {
+  return type == MFB200_TYPE_F32    ? __uint_as_float(bits)
+         : type == MFB200_TYPE_BF16 ? __uint_as_float(bits << 16)
+                                    : __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
 }
 
 __device__ __forceinline__ const void *row_of(const void *base, int type, long long stride, int b) {
@@ -158,8 +162,28 @@ __device__ __forceinline__ int load_index(const PolicyRows &r, const Moves &m, i
 // path costs more than its bytes, because the fence before a row's copy waits
 // for it too (65536 positions of the clipped loss took 330 us with 280 bytes
 // of spills). The other warps take the positions that this one is late for.
+//
+// Where the warps have several turns, a long list that comes last would keep
+// its CTA waiting (65536 positions: 17 us), so the CTA looks for them first and
+// its warps begin with them; body does not see them then.
+constexpr unsigned kNone = 0xffffffffu;
+constexpr int kLongLists = 64;
+struct Turns {
+  unsigned next;                    // turn that no warp has taken yet
+  int found, taken;                 // long lists
+  unsigned long_rows[kLongLists];
+};
+// Sets the counters; all threads of the CTA. The first three turns of a warp are fixed.
+__device__ __forceinline__ void start_turns(Turns *turns) {
+  if (threadIdx.x == 0) {
+    turns->next = 3 * (blockDim.x >> 5);
+    turns->found = turns->taken = 0;
+  }
+  __syncthreads();
+}
+
 template <class Body, class Rare>
-__device__ __forceinline__ void for_positions(const PolicyRows &r, unsigned ctas, unsigned *next_turn,
+__device__ __forceinline__ void for_positions(const PolicyRows &r, unsigned ctas, Turns *turns,
                                               Body body, Rare rare) {
   const int lane = threadIdx.x & 31;
   const unsigned batch = r.batch;
@@ -169,9 +193,34 @@ __device__ __forceinline__ void for_positions(const PolicyRows &r, unsigned ctas
     return blockIdx.x * warps + (turn & (warps - 1)) + (turn >> shift) * step;
   };
   const int base = r.off[0];
-  // turns of this warp: now, next, after (the first three are fixed)
+  bool long_first = false;
+  if (row(4 * warps) < batch) {
+    for (unsigned t = threadIdx.x; row(t) < batch; t += blockDim.x) {
+      const long long count = static_cast<long long>(r.off[row(t) + 1]) - r.off[row(t)];
+      if (count > 64) {
+        const int i = atomicAdd(&turns->found, 1);
+        if (i < kLongLists) turns->long_rows[i] = row(t);
+      }
+    }
+    __syncthreads();
+    long_first = turns->found <= kLongLists;
+  }
+  auto take_long = [&] {
+    int i = 0;
+    if (lane == 0) i = atomicAdd(&turns->taken, 1);
+    i = __shfl_sync(kFull, i, 0);
+    return long_first && i < turns->found ? turns->long_rows[i] : kNone;
+  };
+  unsigned todo = long_first ? take_long() : kNone;  // for rare
+  // turns of this warp: now, next, after
   unsigned t0 = threadIdx.x >> 5, t1 = t0 + warps, t2 = t1 + warps;
-  while (row(t0) < batch) {
+  while (true) {
+    if (todo != kNone) {
+      rare(static_cast<int>(todo), resolve(r, load_head(r, todo), base));
+      todo = long_first ? take_long() : kNone;
+      continue;
+    }
+    if (row(t0) >= batch) break;
     Moves m = resolve(r, load_head(r, row(t0)), base);
     ListHead next{};
     if (row(t1) < batch) next = load_head(r, row(t1));
@@ -190,8 +239,8 @@ __device__ __forceinline__ void for_positions(const PolicyRows &r, unsigned ctas
         if (row(t2) < batch) after = load_head(r, row(t2));
       }
       unsigned t3 = 0;
-      if (lane == 0) t3 = atomicAdd(next_turn, 1u);
-      turned_down = body(static_cast<int>(b), m, c0, c1);
+      if (lane == 0) t3 = atomicAdd(&turns->next, 1u);
+      turned_down = m.n > 64 ? !long_first : m.bad || body(static_cast<int>(b), m, c0, c1);
       t0 = t1;
       t1 = t2;
       t2 = __shfl_sync(kFull, t3, 0);
@@ -201,13 +250,8 @@ __device__ __forceinline__ void for_positions(const PolicyRows &r, unsigned ctas
       c1 = n1;
       next = after;
     }
-    if (turned_down) rare(static_cast<int>(b), resolve(r, load_head(r, b), base));
+    if (turned_down) todo = b;
   }
-}
-// Sets the counter behind the fixed turns; all threads of the CTA.
-__device__ __forceinline__ void start_turns(unsigned *next_turn) {
-  if (threadIdx.x == 0) *next_turn = 3 * (blockDim.x >> 5);
-  __syncthreads();
 }
 
 // ------------------------------------------------------------------ softmax of a list
@@ -231,14 +275,23 @@ __device__ __forceinline__ void columns(const PolicyRows &r, const Moves &m, int
   }
 }
 
-// z[k] from a row of logits; groups past the list's end are not loaded.
+// Logits of the lane's moves, in two steps: every lane loads (column 0 where it
+// has none, so that no load is in a branch of its own), and no load's value is
+// looked at before the last is under way. Groups past the list's end are not loaded.
 template <int G>
-__device__ __forceinline__ void load_logits(const Moves &m, const void *row, int type,
-                                            const int (&col)[G], float (&z)[G]) {
+__device__ __forceinline__ void load_logits(int n, const void *row, int type, const int (&col)[G],
+                                            unsigned (&bits)[G]) {
+#pragma unroll
+  for (int k = 0; k < G; ++k)
+    if (32 * k < n) bits[k] = load_bits(row, type, max(col[k], 0));
+}
+template <int G>
+__device__ __forceinline__ void logits_of(int n, int type, const int (&col)[G],
+                                          const unsigned (&bits)[G], float (&z)[G]) {
 #pragma unroll
   for (int k = 0; k < G; ++k) {
     z[k] = col[k] == kNoMove ? -INFINITY : 0.0f;
-    if (32 * k < m.n && col[k] >= 0) z[k] = load_logit(row, type, col[k]);
+    if (32 * k < n && col[k] >= 0) z[k] = value_of(type, bits[k]);
   }
 }
 
@@ -491,7 +544,9 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, float inv_te
                                                float *entropy, float *row_state) {
   Edges<G> v;
   columns<G>(r, m, c0, c1, lane, v);
-  load_logits<G>(m, row_of(r.logits, r.type, r.stride, b), r.type, v.col, v.z);
+  unsigned bits[G];
+  load_logits<G>(m.n, row_of(r.logits, r.type, r.stride, b), r.type, v.col, bits);
+  logits_of<G>(m.n, r.type, v.col, bits, v.z);
   float es;
   Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, inv_temp2, lane, v.e, es);
   float none = 0.0f;
@@ -519,16 +574,15 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, float inv_te
 __global__ void __launch_bounds__(32 * kMaxWarps)
     move_logprobs_kernel(const __grid_constant__ PolicyRows r, float *move_logp, float *played_logp, float *entropy,
                          float *row_state) {
-  __shared__ unsigned next_turn;
-  start_turns(&next_turn);
+  __shared__ Turns turns;
+  start_turns(&turns);
   pdl_wait();
   pdl_launch();
   const int lane = threadIdx.x & 31;
   const float inv_temp2 = r.inv_temp * kLog2e;
   for_positions(
-      r, gridDim.x, &next_turn,
+      r, gridDim.x, &turns,
       [&](int b, const Moves &m, int c0, int c1) {
-        if (m.n > 64) return true;
         score_position<2>(r, inv_temp2, b, m, c0, c1, lane, move_logp, played_logp, entropy, row_state);
         return false;
       },
@@ -561,7 +615,8 @@ __device__ __forceinline__ void back_position(const PolicyRows &r, const BackArg
                                               int c1, int lane, RowImage &im) {
   Edges<G> v;
   columns<G>(r, m, c0, c1, lane, v);
-  load_logits<G>(m, row_of(r.logits, r.type, r.stride, b), r.type, v.col, v.z);
+  unsigned bits[G];
+  load_logits<G>(m.n, row_of(r.logits, r.type, r.stride, b), r.type, v.col, bits);
   float g[G], total = 0.0f;
 #pragma unroll
   for (int k = 0; k < G; ++k) {
@@ -570,6 +625,7 @@ __device__ __forceinline__ void back_position(const PolicyRows &r, const BackArg
   }
   const float ga = a.played && m.played >= 0 ? a.played[b] : 0.0f;
   const float gh = a.entropy ? a.entropy[b] : 0.0f;
+  logits_of<G>(m.n, r.type, v.col, bits, v.z);
   float es;
   Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, inv_temp2, lane, v.e, es);
   const float h = softmax_done<false>(q, es, q, total, lane);
@@ -642,8 +698,8 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3)
   const int row_bytes = r.classes * (a.out.type == MFB200_TYPE_F32 ? 4 : 2);
   const unsigned ctas = gridDim.x - (a.total ? 1 : 0);
   RowImage im = clear_image(images + (threadIdx.x >> 5) * image_bytes(row_bytes), row_bytes, lane);
-  __shared__ unsigned next_turn;
-  start_turns(&next_turn);
+  __shared__ Turns turns;
+  start_turns(&turns);
   pdl_wait();
   pdl_launch();
   if (blockIdx.x == ctas) {
@@ -652,9 +708,8 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3)
   }
   const float inv_temp2 = r.inv_temp * kLog2e;
   for_positions(
-      r, ctas, &next_turn,
+      r, ctas, &turns,
       [&](int b, const Moves &m, int c0, int c1) {
-        if (m.n > 64 || m.bad) return true;
         back_position<2>(r, a, inv_temp2, b, m, c0, c1, lane, im);
         return false;
       },
@@ -704,12 +759,15 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
                                               int c1, int lane, RowImage &im) {
   Edges<G> v;
   columns<G>(r, m, c0, c1, lane, v);
-  const void *row = row_of(r.logits, r.type, r.stride, b);
-  load_logits<G>(m, row, r.type, v.col, v.z);
   float d[G];  // the reference's logits, then d = log p - log q
-  if (a.ref) load_logits<G>(m, row_of(a.ref, a.ref_type, a.ref_stride, b), a.ref_type, v.col, d);
+  unsigned bits[G], ref_bits[G];
+  load_logits<G>(m.n, row_of(r.logits, r.type, r.stride, b), r.type, v.col, bits);
+  if (a.ref)
+    load_logits<G>(m.n, row_of(a.ref, a.ref_type, a.ref_stride, b), a.ref_type, v.col, ref_bits);
   const float old = a.old_logp[b], adv = a.advantage[b];
   const float c = a.scale * (a.weight ? a.weight[b] : 1.0f);
+  logits_of<G>(m.n, r.type, v.col, bits, v.z);
+  if (a.ref) logits_of<G>(m.n, a.ref_type, v.col, ref_bits, d);
   float es;
   Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, inv_temp2, lane, v.e, es);
   float h, kl = 0.0f;
@@ -738,7 +796,7 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   const float border = static_cast<float>(adv > 0.0f ? a.high : a.low);
   bool active = adv > 0.0f ? !(ratio > border) : !(ratio < border);
   if (takes && fabsf(ratio - border) <=
-                   border * (4e-6f + 1e-6f * (fabsf(sa) + q.log_s + fabsf(old)))) {
+                   border * (4e-6f + 3e-7f * (fabsf(sa) + q.log_s + fabsf(old)))) {
     if (!kExact) return true;
     double sum = 0.0;
 #pragma unroll
@@ -789,15 +847,14 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3)
     const int row_bytes = r.classes * (a.grad.type == MFB200_TYPE_F32 ? 4 : 2);
     im = clear_image(images + (threadIdx.x >> 5) * image_bytes(row_bytes), row_bytes, lane);
   }
-  __shared__ unsigned next_turn;
-  start_turns(&next_turn);
+  __shared__ Turns turns;
+  start_turns(&turns);
   pdl_wait();
   pdl_launch();
   const float inv_temp2 = r.inv_temp * kLog2e;
   for_positions(
-      r, gridDim.x, &next_turn,
+      r, gridDim.x, &turns,
       [&](int b, const Moves &m, int c0, int c1) {
-        if (m.n > 64 || m.bad) return true;
         return clip_position<2, false>(r, a, inv_temp2, b, m, c0, c1, lane, im);
       },
       [&](int b, const Moves &m) {
