@@ -23,9 +23,9 @@
 // their SM and their warps take positions in turn, the lists of the next ones
 // loaded ahead. A gradient row is put together in shared memory and written by
 // one bulk copy, while the warp goes on. 65536 positions, 1858 fp32 classes, on
-// B200: clipped loss with KL 132 us (615 MB of DRAM traffic; the same reads and
-// copies without any arithmetic 127 us, the copies alone 92), its backward pass
-// alone 111 us, log-probabilities 39 us.
+// B200: clipped loss with KL 128 us (615 MB of DRAM traffic; the same reads and
+// copies without any arithmetic 127 us, the copies alone 92), the backward pass
+// alone 111 us, log-probabilities 32 us.
 #include "policy.cuh"
 
 #include <atomic>
@@ -46,7 +46,7 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kMaxMoves = 256;  // moves of a position that count, as in priors_kernel
-constexpr int kMaxWarps = 8;    // positions per CTA at a time
+constexpr int kMaxWarps = 8;    // of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Inputs are read with ordinary or volatile loads, never as read-only (__ldg,
@@ -275,23 +275,24 @@ __device__ __forceinline__ void columns(const PolicyRows &r, const Moves &m, int
   }
 }
 
-// Logits of the lane's moves, in two steps: every lane loads (column 0 where it
-// has none, so that no load is in a branch of its own), and no load's value is
-// looked at before the last is under way. Groups past the list's end are not loaded.
+// Logits of the lane's moves, in two steps: with two groups every lane loads
+// (column 0 where it has none, so that no load is in a branch of its own), and
+// no load's value is looked at before the last is under way. Eight groups have
+// no registers to spare for that. Groups past the list's end are not loaded.
 template <int G>
 __device__ __forceinline__ void load_logits(int n, const void *row, int type, const int (&col)[G],
                                             unsigned (&bits)[G]) {
 #pragma unroll
   for (int k = 0; k < G; ++k)
-    if (32 * k < n) bits[k] = load_bits(row, type, max(col[k], 0));
+    if (G <= 2 && 32 * k < n) bits[k] = load_bits(row, type, max(col[k], 0));
 }
 template <int G>
-__device__ __forceinline__ void logits_of(int n, int type, const int (&col)[G],
+__device__ __forceinline__ void logits_of(int n, const void *row, int type, const int (&col)[G],
                                           const unsigned (&bits)[G], float (&z)[G]) {
 #pragma unroll
   for (int k = 0; k < G; ++k) {
     z[k] = col[k] == kNoMove ? -INFINITY : 0.0f;
-    if (32 * k < n && col[k] >= 0) z[k] = value_of(type, bits[k]);
+    if (32 * k < n && col[k] >= 0) z[k] = value_of(type, G <= 2 ? bits[k] : load_bits(row, type, col[k]));
   }
 }
 
@@ -385,12 +386,15 @@ __device__ __forceinline__ float softmax_done(Norm &q, float es, Norm &w, float 
   return q.log_s - es * q.inv_s;
 }
 
-// The value of move j, which every lane gets.
+// The value of move j, which every lane gets. Its lane picks it out with a test
+// of every group: a choice among the groups' addresses would put the array into
+// local memory.
 template <int G>
-__device__ __forceinline__ float of_move(const float (&v)[G], int j) {
-  float t = v[0];
+__device__ __forceinline__ float of_move(const float (&v)[G], int j, int lane) {
+  float t = 0.0f;
 #pragma unroll
-  for (int k = 1; k < G; ++k) t = j >> 5 == k ? v[k] : t;
+  for (int k = 0; k < G; ++k)
+    if (32 * k + lane == j) t = v[k];
   return __shfl_sync(kFull, t, j & 31);
 }
 
@@ -545,8 +549,9 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, float inv_te
   Edges<G> v;
   columns<G>(r, m, c0, c1, lane, v);
   unsigned bits[G];
-  load_logits<G>(m.n, row_of(r.logits, r.type, r.stride, b), r.type, v.col, bits);
-  logits_of<G>(m.n, r.type, v.col, bits, v.z);
+  const void *row = row_of(r.logits, r.type, r.stride, b);
+  load_logits<G>(m.n, row, r.type, v.col, bits);
+  logits_of<G>(m.n, row, r.type, v.col, bits, v.z);
   float es;
   Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, inv_temp2, lane, v.e, es);
   float none = 0.0f;
@@ -562,7 +567,7 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, float inv_te
       for (int j = m.n + lane; j < m.count; j += 32) move_logp[m.lo + j] = -INFINITY;
   }
   const bool takes = q.live && m.played >= 0;
-  const float z = of_move<G>(v.z, m.played < 0 ? 0 : m.played);
+  const float z = of_move<G>(v.z, m.played < 0 ? 0 : m.played, lane);
   if (lane == 0) {
     if (played_logp)
       played_logp[b] = m.bad ? quiet_nan() : takes ? (z - q.top) * r.inv_temp - q.log_s : 0.0f;
@@ -616,7 +621,8 @@ __device__ __forceinline__ void back_position(const PolicyRows &r, const BackArg
   Edges<G> v;
   columns<G>(r, m, c0, c1, lane, v);
   unsigned bits[G];
-  load_logits<G>(m.n, row_of(r.logits, r.type, r.stride, b), r.type, v.col, bits);
+  const void *row = row_of(r.logits, r.type, r.stride, b);
+  load_logits<G>(m.n, row, r.type, v.col, bits);
   float g[G], total = 0.0f;
 #pragma unroll
   for (int k = 0; k < G; ++k) {
@@ -625,7 +631,7 @@ __device__ __forceinline__ void back_position(const PolicyRows &r, const BackArg
   }
   const float ga = a.played && m.played >= 0 ? a.played[b] : 0.0f;
   const float gh = a.entropy ? a.entropy[b] : 0.0f;
-  logits_of<G>(m.n, r.type, v.col, bits, v.z);
+  logits_of<G>(m.n, row, r.type, v.col, bits, v.z);
   float es;
   Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, inv_temp2, lane, v.e, es);
   const float h = softmax_done<false>(q, es, q, total, lane);
@@ -761,13 +767,14 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   columns<G>(r, m, c0, c1, lane, v);
   float d[G];  // the reference's logits, then d = log p - log q
   unsigned bits[G], ref_bits[G];
-  load_logits<G>(m.n, row_of(r.logits, r.type, r.stride, b), r.type, v.col, bits);
-  if (a.ref)
-    load_logits<G>(m.n, row_of(a.ref, a.ref_type, a.ref_stride, b), a.ref_type, v.col, ref_bits);
+  const void *row = row_of(r.logits, r.type, r.stride, b);
+  load_logits<G>(m.n, row, r.type, v.col, bits);
+  const void *ref = a.ref ? row_of(a.ref, a.ref_type, a.ref_stride, b) : nullptr;
+  if (a.ref) load_logits<G>(m.n, ref, a.ref_type, v.col, ref_bits);
   const float old = a.old_logp[b], adv = a.advantage[b];
   const float c = a.scale * (a.weight ? a.weight[b] : 1.0f);
-  logits_of<G>(m.n, r.type, v.col, bits, v.z);
-  if (a.ref) logits_of<G>(m.n, a.ref_type, v.col, ref_bits, d);
+  logits_of<G>(m.n, row, r.type, v.col, bits, v.z);
+  if (a.ref) logits_of<G>(m.n, ref, a.ref_type, v.col, ref_bits, d);
   float es;
   Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, inv_temp2, lane, v.e, es);
   float h, kl = 0.0f;
@@ -788,7 +795,7 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
     h = softmax_done<false>(q, es, q, kl, lane);
   }
   const bool takes = q.live && m.played >= 0;
-  const float za = of_move<G>(v.z, m.played < 0 ? 0 : m.played);
+  const float za = of_move<G>(v.z, m.played < 0 ? 0 : m.played, lane);
   const float sa = (za - q.top) * r.inv_temp;
   const float ratio = exp2_fast(((sa - old) - q.log_s) * kLog2e);
   // The gradient jumps where the ratio crosses the clip's border, so a ratio
