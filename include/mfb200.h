@@ -150,6 +150,22 @@ MFB200_API int mfb200_evaluate_priors(mfb200_handle *h, const uint64_t *masks, c
                                       float *priors, float *wdl, float *moves_left,
                                       mfb200_timing *timing);
 
+/* Host-buffer evaluation that returns the log-probabilities of each position's
+ * legal moves (the exact softmax of mfb200_move_logprobs at the end of this
+ * file, not the FastExp priors): move_logp [move_offsets[batch] -
+ * move_offsets[0]], -inf past a position's 256th move; played_logp [batch] of
+ * the played move, played[b] being its place in the position's list or -1 for
+ * none (0 is returned); entropy [batch]. Lists as in mfb200_evaluate_priors;
+ * any output may be NULL, and played where played_logp is. What a frozen
+ * network contributes to the losses below. Blocks until the results are in
+ * host memory. No counterpart in the reference. */
+MFB200_API int mfb200_evaluate_logprobs(mfb200_handle *h, const uint64_t *masks,
+                                        const float *values, int batch,
+                                        const int32_t *move_offsets, const int16_t *move_index,
+                                        const int32_t *played, float softmax_temp,
+                                        float *move_logp, float *played_logp, float *entropy,
+                                        float *wdl, float *moves_left, mfb200_timing *timing);
+
 /* One position of a game history, as the encoder reads it from a Position
  * (src/core/position.h): bit i of a bitboard is square i (a1 = 0, h8 = 63). */
 typedef struct mfb200_board {
@@ -300,7 +316,8 @@ MFB200_API const char *mfb200_noalloc_last_error(void);
  * synchronising. The calls allocate nothing, keep nothing between calls and
  * can be captured into a CUDA graph; calls on different streams or threads do
  * not share anything but the buffers they are given. Results do not depend on
- * timing: the same inputs give the same bits. Returns 0 on success;
+ * timing: the same inputs give the same bits. Outputs may not overlap inputs or
+ * one another. Returns 0 on success;
  * mfb200_policy_last_error() gives the calling thread's last message.
  *
  * The softmax of a position runs over its first n = min(count, 256) listed
@@ -310,8 +327,8 @@ MFB200_API const char *mfb200_noalloc_last_error(void);
  * twice, and its column gets the sum of both gradients. Columns that are not
  * listed are never read, whatever they hold. A position without a legal move
  * (empty list, or every listed logit -inf) takes part in nothing: zero losses,
- * zero gradients, log-probability 0 for its played move and -inf for listed
- * ones. A NaN or +inf among the listed logits makes the position's results
+ * gradients, KL and entropy, log-probability 0 for its played move and -inf for
+ * listed ones. A NaN or +inf among the listed logits makes the position's results
  * NaN. A position whose offsets decrease or reach outside [0, num_moves], or
  * whose played move is below -1 or not among its n moves, is not read past its
  * list: its per-position results and its whole gradient row are NaN. Sums and

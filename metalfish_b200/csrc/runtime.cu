@@ -40,6 +40,7 @@
 #include "../../include/mfb200_testing.h"
 #include "gemm_host.h"
 #include "kernels.cuh"
+#include "policy.cuh"
 
 using namespace mfb200;
 
@@ -287,7 +288,9 @@ struct Shard {  // one GPU
   float *policy, *wdl, *mlh;
   int32_t *move_off;      // legal-move priors: CSR offsets [max_batch + 1]
   int16_t *move_idx;      //   policy index per legal move [max_batch * 256]
-  float *priors;          //   priors per legal move [max_batch * 256]
+  float *priors;          //   priors (or log-probabilities) per legal move [max_batch * 256]
+  int32_t *played;        // log-probabilities: the played move of each position [max_batch]
+  float *played_logp, *entropy;  //   per position [max_batch]
   mfb200_board *boards;   // encoder input: history records [max_batch * 128]
   int32_t *hist_off;      //   CSR offsets [max_batch + 1]
   int32_t *transforms;    //   canonicalisation transform per position [max_batch]
@@ -715,6 +718,9 @@ void alloc_workspace(Shard &S, const mfb200_net_desc &n, int max_batch, bool fp8
       {reinterpret_cast<void **>(&S.move_off), (B + 1) * 4},
       {reinterpret_cast<void **>(&S.move_idx), B * kMoveCapacity * 2},
       {reinterpret_cast<void **>(&S.priors), B * kMoveCapacity * 4},
+      {reinterpret_cast<void **>(&S.played), B * 4},
+      {reinterpret_cast<void **>(&S.played_logp), B * 4},
+      {reinterpret_cast<void **>(&S.entropy), B * 4},
       {reinterpret_cast<void **>(&S.boards), B * kHistoryCapacity * sizeof(mfb200_board)},
       {reinterpret_cast<void **>(&S.hist_off), (B + 1) * 4},
       {reinterpret_cast<void **>(&S.transforms), B * 4},
@@ -1446,6 +1452,58 @@ int eval_shard_priors(mfb200_handle *h, Shard &S, const uint64_t *masks, const f
   cudaEventElapsedTime(&ms[3], S.ev[0], S.ev[3]);
   return 0;
 }
+// The forward followed by the legal moves' log-probabilities of the shard's
+// positions; the CSR arrays are slices as in eval_shard_priors, the per-position
+// arrays the shard's own.
+int eval_shard_logprobs(mfb200_handle *h, Shard &S, const uint64_t *masks, const float *values,
+                        int B, const int32_t *offsets, const int16_t *index, const int32_t *played,
+                        float temp, float *move_logp, float *played_logp, float *entropy,
+                        float *wdl, float *mlh, float *ms) {
+  check(cudaSetDevice(S.device), "cudaSetDevice");
+  cudaStream_t s = S.stream;
+  const int32_t nmoves = offsets[B] - offsets[0];
+  check(cudaEventRecord(S.ev[0], s), "event");
+  check(cudaMemcpyAsync(S.masks, masks, size_t(B) * kPlanes * 8, cudaMemcpyHostToDevice, s), "H2D masks");
+  check(cudaMemcpyAsync(S.values, values, size_t(B) * kPlanes * 4, cudaMemcpyHostToDevice, s), "H2D values");
+  check(cudaMemcpyAsync(S.move_off, offsets, size_t(B + 1) * 4, cudaMemcpyHostToDevice, s), "H2D offsets");
+  if (nmoves > 0)
+    check(cudaMemcpyAsync(S.move_idx, index, size_t(nmoves) * 2, cudaMemcpyHostToDevice, s), "H2D moves");
+  if (played)
+    check(cudaMemcpyAsync(S.played, played, size_t(B) * 4, cudaMemcpyHostToDevice, s), "H2D played");
+  check(cudaEventRecord(S.ev[1], s), "event");
+  forward(h, S, B, s);
+  PolicyRows r{};
+  r.logits = S.policy;
+  r.stride = kPolicy;
+  r.type = MFB200_TYPE_F32;
+  r.batch = B;
+  r.classes = kPolicy;
+  r.off = S.move_off;
+  r.index = S.move_idx;
+  r.num_moves = nmoves;
+  r.played = played ? S.played : nullptr;
+  r.temp = temp;
+  r.inv_temp = static_cast<float>(1.0 / temp);
+  check(launch_move_logprobs(r, move_logp ? S.priors : nullptr, played ? S.played_logp : nullptr,
+                             S.entropy, nullptr, s),
+        "log-probabilities launch");
+  check(cudaEventRecord(S.ev[2], s), "event");
+  if (move_logp && nmoves > 0)
+    check(cudaMemcpyAsync(move_logp, S.priors, size_t(nmoves) * 4, cudaMemcpyDeviceToHost, s), "D2H log-probabilities");
+  if (played_logp)
+    check(cudaMemcpyAsync(played_logp, S.played_logp, size_t(B) * 4, cudaMemcpyDeviceToHost, s), "D2H played");
+  if (entropy) check(cudaMemcpyAsync(entropy, S.entropy, size_t(B) * 4, cudaMemcpyDeviceToHost, s), "D2H entropy");
+  if (wdl) check(cudaMemcpyAsync(wdl, S.wdl, size_t(B) * 12, cudaMemcpyDeviceToHost, s), "D2H wdl");
+  if (mlh) check(cudaMemcpyAsync(mlh, S.mlh, size_t(B) * 4, cudaMemcpyDeviceToHost, s), "D2H mlh");
+  check(cudaEventRecord(S.ev[3], s), "event");
+  check(cudaStreamSynchronize(s), "forward");
+  check_status(S);
+  cudaEventElapsedTime(&ms[0], S.ev[0], S.ev[1]);
+  cudaEventElapsedTime(&ms[1], S.ev[1], S.ev[2]);
+  cudaEventElapsedTime(&ms[2], S.ev[2], S.ev[3]);
+  cudaEventElapsedTime(&ms[3], S.ev[0], S.ev[3]);
+  return 0;
+}
 // Upload one shard's histories and encode them into S.masks / S.values.
 void encode_shard(Shard &S, const mfb200_board *boards, const int32_t *offsets, int B, int fmt,
                   cudaStream_t s) {
@@ -1853,6 +1911,77 @@ extern "C" int mfb200_evaluate_priors(mfb200_handle *h, const uint64_t *masks,
   }
   for (auto &e : errs)
     if (!e.empty()) return fail(h, "mfb200_evaluate_priors: " + e);
+  if (timing) {
+    *timing = mfb200_timing{0, 0, 0, 0};
+    for (auto &m : ms) {
+      timing->h2d_ms = std::max(timing->h2d_ms, m[0]);
+      timing->forward_ms = std::max(timing->forward_ms, m[1]);
+      timing->d2h_ms = std::max(timing->d2h_ms, m[2]);
+      timing->total_ms = std::max(timing->total_ms, m[3]);
+    }
+  }
+  return 0;
+}
+
+extern "C" int mfb200_evaluate_logprobs(mfb200_handle *h, const uint64_t *masks,
+                                        const float *values, int batch,
+                                        const int32_t *move_offsets, const int16_t *move_index,
+                                        const int32_t *played, float softmax_temp,
+                                        float *move_logp, float *played_logp, float *entropy,
+                                        float *wdl, float *mlh, mfb200_timing *timing) {
+  if (!h) return fail(nullptr, "mfb200_evaluate_logprobs: null handle");
+  std::lock_guard<std::mutex> lock(h->mu);
+  if (batch <= 0) return 0;
+  if (batch > h->cfg.max_batch)
+    return fail(h, "mfb200_evaluate_logprobs: batch " + std::to_string(batch) +
+                       " exceeds max_batch " + std::to_string(h->cfg.max_batch));
+  if (!masks || !values || !move_offsets || (!move_index && move_offsets[batch] != move_offsets[0]))
+    return fail(h, "mfb200_evaluate_logprobs: null input");
+  if (played_logp && !played) return fail(h, "mfb200_evaluate_logprobs: played_logp needs played");
+  if (!(softmax_temp >= 1e-30f && softmax_temp <= 1e30f))
+    return fail(h, "mfb200_evaluate_logprobs: softmax_temp must be positive (between 1e-30 and 1e30)");
+  for (int b = 0; b < batch; ++b) {
+    if (move_offsets[b + 1] < move_offsets[b])
+      return fail(h, "mfb200_evaluate_logprobs: move_offsets must be non-decreasing");
+    const int64_t n = std::min<int64_t>(int64_t(move_offsets[b + 1]) - move_offsets[b], 256);
+    if (played && (played[b] < -1 || played[b] >= n))
+      return fail(h, "mfb200_evaluate_logprobs: played must be -1 or one of the position's first 256 moves");
+  }
+  const int nd = static_cast<int>(h->shards.size());
+  const int per = (batch + nd - 1) / nd;
+  for (int i = 0; i < nd; ++i) {
+    const int lo = i * per, hi = std::min(batch, lo + per);
+    if (lo < hi && int64_t(move_offsets[hi]) - move_offsets[lo] > int64_t(per) * kMoveCapacity)
+      return fail(h, "mfb200_evaluate_logprobs: more than " + std::to_string(kMoveCapacity) +
+                         " legal moves per position on average");
+  }
+  std::vector<std::array<float, 4>> ms(nd, {0, 0, 0, 0});
+  std::vector<std::string> errs(nd);
+  auto work = [&](int i) {
+    const int lo = i * per, hi = std::min(batch, lo + per);
+    if (lo >= hi) return;
+    const int32_t base = move_offsets[lo] - move_offsets[0];
+    try {
+      eval_shard_logprobs(h, *h->shards[i], masks + size_t(lo) * kPlanes,
+                          values + size_t(lo) * kPlanes, hi - lo, move_offsets + lo,
+                          move_index ? move_index + base : nullptr, played ? played + lo : nullptr,
+                          softmax_temp, move_logp ? move_logp + base : nullptr,
+                          played_logp ? played_logp + lo : nullptr, entropy ? entropy + lo : nullptr,
+                          wdl ? wdl + size_t(lo) * 3 : nullptr, mlh ? mlh + lo : nullptr,
+                          ms[i].data());
+    } catch (const std::exception &e) {
+      errs[i] = e.what();
+    }
+  };
+  if (nd == 1) {
+    work(0);
+  } else {
+    std::vector<std::thread> th;
+    for (int i = 0; i < nd; ++i) th.emplace_back(work, i);
+    for (auto &t : th) t.join();
+  }
+  for (auto &e : errs)
+    if (!e.empty()) return fail(h, "mfb200_evaluate_logprobs: " + e);
   if (timing) {
     *timing = mfb200_timing{0, 0, 0, 0};
     for (auto &m : ms) {

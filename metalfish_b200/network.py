@@ -63,6 +63,9 @@ def _declare(L):
     L.mfb200_evaluate_priors.restype = c_int
     L.mfb200_evaluate_priors.argtypes = [vp, vp, vp, c_int, vp, vp, ctypes.c_float, vp, vp, vp,
                                          ctypes.POINTER(Timing)]
+    L.mfb200_evaluate_logprobs.restype = c_int
+    L.mfb200_evaluate_logprobs.argtypes = [vp, vp, vp, c_int, vp, vp, vp, ctypes.c_float, vp, vp, vp,
+                                           vp, vp, ctypes.POINTER(Timing)]
     L.mfb200_encode_history.restype = c_int
     L.mfb200_encode_history.argtypes = [vp, vp, vp, c_int, c_int, vp, vp, vp]
     L.mfb200_evaluate_history.restype = c_int
@@ -223,6 +226,41 @@ class B200Network:
         if rc != 0:
             raise self._err()
         return pri, wdl, mlh
+
+    def evaluate_logprobs(self, inp: PackedInputs, move_offsets: np.ndarray, move_index: np.ndarray,
+                          played: Optional[np.ndarray] = None, softmax_temp: float = 1.0,
+                          timing: Optional[Timing] = None):
+        """Forward plus the exact log-probabilities of the legal moves on the GPU
+        (``metalfish_b200.policy.move_logprobs`` on this network's logits): lists
+        as in evaluate_priors, played [B] the played move's place in its
+        position's list or -1. Returns (move_logp [moves], played_logp [B] or
+        None, entropy [B], wdl [B, 3], moves_left [B])."""
+        b = inp.count
+        masks = np.ascontiguousarray(inp.masks, np.uint64)
+        values = np.ascontiguousarray(inp.values, np.float32)
+        off = np.ascontiguousarray(move_offsets, np.int32)
+        idx = np.ascontiguousarray(move_index, np.int16)
+        if off.shape != (b + 1,):
+            raise ValueError("move_offsets must have batch + 1 entries")
+        if idx.size < int(off[-1]) - int(off[0]):
+            raise ValueError("move_index is shorter than move_offsets says")
+        pl = None if played is None else np.ascontiguousarray(played, np.int32)
+        if pl is not None and pl.shape != (b,):
+            raise ValueError("played must have one entry per position")
+        logp = np.empty(max(int(off[-1]) - int(off[0]), 0), np.float32)
+        at = None if pl is None else np.empty(b, np.float32)
+        ent = np.empty(b, np.float32)
+        wdl = np.empty((b, 3), np.float32)
+        mlh = np.empty(b, np.float32)
+        rc = _lib().mfb200_evaluate_logprobs(
+            self._h, masks.ctypes.data, values.ctypes.data, b, off.ctypes.data,
+            idx.ctypes.data if idx.size else None, None if pl is None else pl.ctypes.data,
+            ctypes.c_float(softmax_temp), logp.ctypes.data, None if at is None else at.ctypes.data,
+            ent.ctypes.data, wdl.ctypes.data, mlh.ctypes.data,
+            ctypes.byref(timing) if timing is not None else None)
+        if rc != 0:
+            raise self._err()
+        return logp, at, ent, wdl, mlh
 
     # -- position encoding on the GPU (board records: include/mfb200.h mfb200_board,
     #    112 bytes each, as uint8 rows or a structured array)
