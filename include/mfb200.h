@@ -314,7 +314,7 @@ MFB200_API const char *mfb200_noalloc_last_error(void);
  * pointer of the current device (the logits' device is checked); the work is
  * enqueued on `stream` (a cudaStream_t, NULL = legacy default stream) without
  * synchronising. The calls allocate nothing, keep nothing between calls and
- * can be captured into a CUDA graph; calls on different streams or threads do
+ * can be captured into a CUDA graph (make a first call on the device before); calls on different streams or threads do
  * not share anything but the buffers they are given. Results do not depend on
  * timing: the same inputs give the same bits. Outputs may not overlap inputs or
  * one another. Returns 0 on success;
@@ -393,7 +393,9 @@ typedef struct {
  * Outputs, each may be NULL: d_loss, d_logp (0 without a played move), d_kl,
  * d_entropy [batch]; d_total [1], the sum of d_loss (needs d_loss);
  * d_grad_logits as in mfb200_move_logprobs_backward. A reference logit of -inf
- * at a move that the policy gives a probability makes the KL infinite. */
+ * at a move that the policy gives a probability makes the KL infinite (and the
+ * gradient of the row infinite or NaN, as the formula is); a reference without
+ * any move above -inf, or with NaN or +inf among them, makes it NaN. */
 MFB200_API int mfb200_clipped_policy_loss(const mfb200_policy_rows *rows,
                                           const mfb200_clip_config *cfg, const float *d_old_logp,
                                           const float *d_advantage, const float *d_weight,

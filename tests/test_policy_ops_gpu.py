@@ -404,6 +404,24 @@ def test_nan_and_infinity_among_listed_logits_stay_in_their_row():
     assert (got.grad_logits[1].cpu()[off] == 0).all()
 
 
+def test_reference_without_a_move_makes_the_kl_infinite():
+    x = Batch("f32", 1858, [40] * 4, 27)
+    x.played_host[:] = 3
+    x.played.fill_(3)
+    other = x.logits.clone()
+    other[1, int(x.lists[1][9])] = -np.inf
+    x.logits[2, int(x.lists[2][9])] = -np.inf  # the policy does not play it either: no term
+    other[2, int(x.lists[2][9])] = -np.inf
+    other[3, int(x.lists[3][9])] = float("nan")
+    zero, one = torch.zeros(4, device="cuda"), torch.ones(4, device="cuda")
+    out = policy.clipped_policy_loss(*x.args(), zero - 3, one, ref_logits=other, kl_coef=0.1)
+    kl = out.kl.cpu().numpy()
+    assert kl[0] == 0 and kl[1] == np.inf and abs(kl[2]) < 1e-6 and np.isnan(kl[3])
+    assert np.isinf(out.loss[1].item())
+    for b in (0, 2):
+        assert torch.isfinite(out.grad_logits[b]).all() and torch.isfinite(out.loss[b])
+
+
 @pytest.mark.parametrize("case", ["decreasing", "beyond", "before", "played high", "played low"])
 def test_malformed_positions_are_nan_and_alone(case):
     """Lists that decrease or reach outside the indices, played moves that are
