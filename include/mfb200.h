@@ -156,7 +156,8 @@ MFB200_API int mfb200_evaluate_priors(mfb200_handle *h, const uint64_t *masks, c
  * move_offsets[0]], -inf past a position's 256th move; played_logp [batch] of
  * the played move, played[b] being its place in the position's list or -1 for
  * none (0 is returned); entropy [batch]. Lists as in mfb200_evaluate_priors;
- * any output may be NULL, and played where played_logp is. What a frozen
+ * any output may be NULL, and played where played_logp is; softmax_temp lies
+ * between 1e-30 and 1e30. What a frozen
  * network contributes to the losses below. Blocks until the results are in
  * host memory. No counterpart in the reference. */
 MFB200_API int mfb200_evaluate_logprobs(mfb200_handle *h, const uint64_t *masks,

@@ -163,9 +163,9 @@ __device__ __forceinline__ int load_index(const PolicyRows &r, const Moves &m, i
 // for it too (65536 positions of the clipped loss took 330 us with 280 bytes
 // of spills). The other warps take the positions that this one is late for.
 //
-// Where the warps have several turns, a long list that comes last would keep
-// its CTA waiting (65536 positions: 17 us), so the CTA looks for them first and
-// its warps begin with them; body does not see them then.
+// Where some warps have more than two turns, a long list that comes last would
+// keep its CTA waiting (65536 positions: 17 us), so the CTA looks for them first
+// and its warps begin with them; body does not see them then.
 constexpr unsigned kNone = 0xffffffffu;
 constexpr int kLongLists = 64;
 struct Turns {
@@ -194,7 +194,7 @@ __device__ __forceinline__ void for_positions(const PolicyRows &r, unsigned ctas
   };
   const int base = r.off[0];
   bool long_first = false;
-  if (row(4 * warps) < batch) {
+  if (row(2 * warps) < batch) {
     for (unsigned t = threadIdx.x; row(t) < batch; t += blockDim.x) {
       const long long count = static_cast<long long>(r.off[row(t) + 1]) - r.off[row(t)];
       if (count > 64) {

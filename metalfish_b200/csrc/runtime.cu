@@ -1928,7 +1928,7 @@ extern "C" int mfb200_evaluate_logprobs(mfb200_handle *h, const uint64_t *masks,
                                         const int32_t *move_offsets, const int16_t *move_index,
                                         const int32_t *played, float softmax_temp,
                                         float *move_logp, float *played_logp, float *entropy,
-                                        float *wdl, float *mlh, mfb200_timing *timing) {
+                                        float *wdl, float *mlh, mfb200_timing *timing) try {
   if (!h) return fail(nullptr, "mfb200_evaluate_logprobs: null handle");
   std::lock_guard<std::mutex> lock(h->mu);
   if (batch <= 0) return 0;
@@ -1973,13 +1973,17 @@ extern "C" int mfb200_evaluate_logprobs(mfb200_handle *h, const uint64_t *masks,
       errs[i] = e.what();
     }
   };
-  if (nd == 1) {
-    work(0);
-  } else {
-    std::vector<std::thread> th;
-    for (int i = 0; i < nd; ++i) th.emplace_back(work, i);
-    for (auto &t : th) t.join();
+  std::vector<std::thread> th;
+  th.reserve(nd);
+  for (int i = 1; i < nd; ++i) {
+    try {
+      th.emplace_back(work, i);
+    } catch (const std::exception &) {
+      work(i);  // no thread to be had
+    }
   }
+  work(0);
+  for (auto &t : th) t.join();
   for (auto &e : errs)
     if (!e.empty()) return fail(h, "mfb200_evaluate_logprobs: " + e);
   if (timing) {
@@ -1992,6 +1996,8 @@ extern "C" int mfb200_evaluate_logprobs(mfb200_handle *h, const uint64_t *masks,
     }
   }
   return 0;
+} catch (const std::exception &e) {  // no memory for the lists above
+  return fail(h, std::string("mfb200_evaluate_logprobs: ") + e.what());
 }
 
 extern "C" int mfb200_evaluate(mfb200_handle *h, const uint64_t *masks, const float *values,

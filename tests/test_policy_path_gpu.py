@@ -181,3 +181,41 @@ def test_a_step_captured_while_an_eager_graph_lives(setup):
     torch.cuda.synchronize()
     want = policy.clipped_policy_loss(logits, off, idx, played, old, adv).grad_logits
     assert torch.equal(w.grad, want)
+
+
+two = pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+
+
+@two
+def test_two_devices_shard_the_log_probabilities(setup):
+    _, inp, off, idx, played = setup
+    t = synthetic.generate(synthetic.TINY, 11, perturb_norms=True)
+    pair = create_network(synthetic.TINY, t, max_batch=B, num_devices=2)
+    one = create_network(synthetic.TINY, t, max_batch=B)
+    try:
+        got = pair.evaluate_logprobs(inp, off, idx, played)
+        half = B // 2
+        for lo, hi in ((0, half), (half, B)):
+            want = one.evaluate_logprobs(PackedInputs(inp.masks[lo:hi], inp.values[lo:hi]), off[lo:hi + 1],
+                                         idx[off[lo] - off[0]:off[hi] - off[0]], played[lo:hi])
+            np.testing.assert_array_equal(got[0][off[lo] - off[0]:off[hi] - off[0]], want[0])
+            for a, b in zip(got[1:], want[1:]):
+                np.testing.assert_array_equal(a[lo:hi], b)
+    finally:
+        pair.close()
+        one.close()
+
+
+@two
+def test_tensors_on_another_device_than_the_current_one(setup):
+    _, _, off, idx, played = setup
+    logits = torch.randn(B, 1858)
+    args = [torch.from_numpy(a) for a in (off, idx, played)]
+    want = policy.move_logprobs(logits.to("cuda:0"), *[a.to("cuda:0") for a in args])
+    assert torch.cuda.current_device() == 0
+    got = policy.move_logprobs(logits.to("cuda:1"), *[a.to("cuda:1") for a in args])
+    assert torch.cuda.current_device() == 0 and got.moves.device.index == 1
+    for a, b in zip(got, want):
+        assert torch.equal(a.cpu(), b.cpu())
+    with pytest.raises(ValueError, match="cuda:0"):
+        policy.move_logprobs(logits.to("cuda:1"), *[a.to("cuda:0") for a in args])
