@@ -629,6 +629,36 @@ def test_captured_and_replayed_with_new_inputs():
                 assert same(got, want)
 
 
+def test_the_calls_allocate_nothing():
+    """Free device memory is the same after many calls into given buffers."""
+    x = Batch("f32", 1858, [33] * 500, 28)
+    z, one = torch.zeros(500, device="cuda") - 3, torch.ones(500, device="cuda")
+    lines = torch.arange(0, 501, 10, dtype=torch.int32, device="cuda")
+    grad = torch.empty(500, 1858, device="cuda")
+    out = [torch.empty(500, device="cuda") for _ in range(6)]
+    total, moves = torch.empty((), device="cuda"), torch.empty(len(x.flat), device="cuda")
+    L = policy._lib()
+    rows, _ = policy._rows(*x.args(), 1.0)
+    p = [t.data_ptr() for t in out]
+
+    def calls():
+        assert L.mfb200_move_logprobs(rows, moves.data_ptr(), p[0], p[1], None) == 0
+        assert L.mfb200_clipped_policy_loss(
+            rows, policy._ClipConfig(0.2, 0.2, 0.0, 0.1, 1.0), z.data_ptr(), one.data_ptr(), None, None, 0, 0,
+            p[0], p[1], None, p[2], total.data_ptr(), grad.data_ptr(), 1858, 0, None) == 0
+        assert L.mfb200_preference_loss(
+            rows, policy._PreferenceConfig(0.1, 0.0, 1.0), lines.data_ptr(), 25, z.data_ptr(), None, p[0], p[1],
+            p[2], p[3], p[4], total.data_ptr(), grad.data_ptr(), 1858, 0, None) == 0
+
+    calls()
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(50):
+        calls()
+    torch.cuda.synchronize()
+    assert torch.cuda.mem_get_info()[0] == free
+
+
 # ---------------------------------------------------------------- gradients against differences
 
 def test_gradients_against_differences():
