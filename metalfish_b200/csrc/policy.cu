@@ -124,15 +124,16 @@ struct Moves {
   int played;  // edge number, -1 for none
   bool bad;    // offsets or played move out of range
 };
-// No entry outside [0, num_moves) is ever read.
+// No entry outside [0, num_moves) is ever read. (The offsets are in order
+// before their differences are taken, so those are right as unsigned numbers.)
 __device__ __forceinline__ Moves resolve(const PolicyRows &r, const ListHead &head, int base) {
   Moves m;
-  const long long lo = static_cast<long long>(head.lo) - base;
-  const long long hi = static_cast<long long>(head.hi) - base;
-  m.bad = lo < 0 || hi < lo || hi > r.num_moves;
-  m.lo = m.bad ? 0 : static_cast<int>(lo);
+  const unsigned lo = static_cast<unsigned>(head.lo) - static_cast<unsigned>(base);
+  const unsigned hi = static_cast<unsigned>(head.hi) - static_cast<unsigned>(base);
+  m.bad = head.lo < base || head.hi < head.lo || hi > static_cast<unsigned>(r.num_moves);
+  m.lo = static_cast<int>(lo);
   m.count = m.bad ? 0 : static_cast<int>(hi - lo);
-  m.n = m.count < kMaxMoves ? m.count : kMaxMoves;
+  m.n = min(m.count, kMaxMoves);
   // a position with an empty list has no played move, whatever it is given
   m.bad = m.bad || head.played < -1 || (m.count > 0 && head.played >= m.n);
   m.played = m.bad || m.count == 0 ? -1 : head.played;
@@ -212,39 +213,39 @@ __device__ __forceinline__ void for_positions(const PolicyRows &r, unsigned ctas
     return long_first && i < turns->found ? turns->long_rows[i] : kNone;
   };
   unsigned todo = long_first ? take_long() : kNone;  // for rare
-  // turns of this warp: now, next, after
-  unsigned t0 = threadIdx.x >> 5, t1 = t0 + warps, t2 = t1 + warps;
+  // this warp's positions: now, next, after
+  unsigned b0 = row(threadIdx.x >> 5), b1 = b0 + step, b2 = b1 + step;
   while (true) {
     if (todo != kNone) {
       rare(static_cast<int>(todo), resolve(r, load_head(r, todo), base));
       todo = long_first ? take_long() : kNone;
       continue;
     }
-    if (row(t0) >= batch) break;
-    Moves m = resolve(r, load_head(r, row(t0)), base);
+    if (b0 >= batch) break;
+    Moves m = resolve(r, load_head(r, b0), base);
     ListHead next{};
-    if (row(t1) < batch) next = load_head(r, row(t1));
+    if (b1 < batch) next = load_head(r, b1);
     int c0 = load_index(r, m, 0, lane), c1 = m.n > 32 ? load_index(r, m, 1, lane) : -32768;
     unsigned b;
     bool turned_down;
     while (true) {
-      b = row(t0);
+      b = b0;
       Moves mn{};
       int n0 = -32768, n1 = -32768;
       ListHead after{};
-      if (row(t1) < batch) {
+      if (b1 < batch) {
         mn = resolve(r, next, base);
         n0 = load_index(r, mn, 0, lane);
         if (mn.n > 32) n1 = load_index(r, mn, 1, lane);
-        if (row(t2) < batch) after = load_head(r, row(t2));
+        if (b2 < batch) after = load_head(r, b2);
       }
-      unsigned t3 = 0;
-      if (lane == 0) t3 = atomicAdd(&turns->next, 1u);
+      unsigned turn = 0;
+      if (lane == 0) turn = atomicAdd(&turns->next, 1u);
       turned_down = m.n > 64 ? !long_first : m.bad || body(static_cast<int>(b), m, c0, c1);
-      t0 = t1;
-      t1 = t2;
-      t2 = __shfl_sync(kFull, t3, 0);
-      if (turned_down || row(t0) >= batch) break;
+      b0 = b1;
+      b1 = b2;
+      b2 = row(__shfl_sync(kFull, turn, 0));
+      if (turned_down || b0 >= batch) break;
       m = mn;
       c0 = n0;
       c1 = n1;
