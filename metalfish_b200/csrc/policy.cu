@@ -48,6 +48,7 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kMaxMoves = 256;  // moves of a position that count, as in priors_kernel
 constexpr int kMaxWarps = 8;    // of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2eRest = static_cast<float>(1.4426950408889634 - static_cast<double>(kLog2e));
 
 // Inputs are read with ordinary or volatile loads, never as read-only (__ldg,
 // __restrict__ const): a kernel here may start before the one that writes its
@@ -105,6 +106,12 @@ __device__ __forceinline__ float exp2_fast(float t) {
   float v;
   asm("ex2.approx.f32 %0, %1;" : "=f"(v) : "f"(t));
   return v;
+}
+// e^s for s <= 0 as 2^(s log2 e), log2 e in two parts: the rounding of the
+// argument is that of one operation and does not lean to one side, which sums
+// of log-probabilities over long lines would add up.
+__device__ __forceinline__ float exp_fast(float s) {
+  return exp2_fast(fmaf(s, kLog2e, s * kLog2eRest));
 }
 __device__ __forceinline__ float quiet_nan() { return __int_as_float(0x7FC00000); }
 
@@ -308,11 +315,10 @@ struct Norm {
 };
 
 // Largest logit, and e[k] = exp(s - s_top) with this lane's part of `rest` and
-// of sum e s. The exponential is 2^(s log2 e) in one instruction; the rounding
-// of its argument, half a step times |s|, is no more than that of s itself.
+// of sum e s.
 template <int G>
 __device__ __forceinline__ Norm softmax_part(int n, const float (&z)[G], float inv_temp,
-                                             float inv_temp2, int lane, float (&e)[G],
+                                             int lane, float (&e)[G],
                                              float &es) {
   Norm q;
   float top = z[0];
@@ -336,9 +342,9 @@ __device__ __forceinline__ Norm softmax_part(int n, const float (&z)[G], float i
     if (32 * k < n) {
       const unsigned at = __ballot_sync(kFull, z[k] == q.top);
       if (q.lead < 0 && at) q.lead = 32 * k + __ffs(at) - 1;
-      const float d = z[k] - q.top;
-      e[k] = exp2_fast(d * inv_temp2);
-      if (e[k] != 0.0f) es += e[k] * (d * inv_temp);
+      const float t = (z[k] - q.top) * inv_temp;
+      e[k] = exp_fast(t);
+      if (e[k] != 0.0f) es += e[k] * t;
       if (32 * k + lane != q.lead) q.rest += e[k];
     }
   }
@@ -544,8 +550,13 @@ __device__ __forceinline__ void write_nan_row(const Grad &out, int classes, int 
 }
 
 // ------------------------------------------------------------------ log-probabilities
-template <int G>
-__device__ __forceinline__ void score_position(const PolicyRows &r, float inv_temp2, int b,
+// kLines: the played move's log-probability goes into sums over long lines whose
+// differences are small, where what leans to one side adds up (the fast
+// exponential and the rounding of 1 / T do, by some 1e-8): it is made from the
+// accurate exponential, 1 / T in two parts and a 64-bit logarithm, and rounded
+// once. row_state is then set.
+template <int G, bool kLines>
+__device__ __forceinline__ void score_position(const PolicyRows &r, int b,
                                                const Moves &m, int c0, int c1, int lane,
                                                float *move_logp, float *played_logp,
                                                float *entropy, float *row_state) {
@@ -556,7 +567,7 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, float inv_te
   load_logits<G>(m.n, row, r.type, v.col, bits);
   logits_of<G>(m.n, row, r.type, v.col, bits, v.z);
   float es;
-  Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, inv_temp2, lane, v.e, es);
+  Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, lane, v.e, es);
   float none = 0.0f;
   const float h = softmax_done<false>(q, es, q, none, lane);
   if (move_logp) {
@@ -571,17 +582,31 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, float inv_te
   }
   const bool takes = q.live && m.played >= 0;
   const float z = of_move<G>(v.z, m.played < 0 ? 0 : m.played, lane);
+  float logp = (z - q.top) * r.inv_temp - q.log_s;
+  if (kLines) {
+    float rest = 0.0f;
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+      if (32 * k < m.n && 32 * k + lane != q.lead) {
+        const float d = v.z[k] - q.top;
+        if (!(d == -INFINITY)) rest += expf(fmaf(d, r.inv_temp, d * r.inv_temp_rest));
+      }
+    rest = warp_sum(rest);
+    if (q.top < INFINITY)  // (else it is NaN already)
+      logp = static_cast<float>((static_cast<double>(z) - q.top) / r.temp - log(1.0 + rest));
+  }
   if (lane == 0) {
-    if (played_logp)
-      played_logp[b] = m.bad ? quiet_nan() : takes ? (z - q.top) * r.inv_temp - q.log_s : 0.0f;
+    if (played_logp) played_logp[b] = m.bad ? quiet_nan() : takes ? logp : 0.0f;
     if (entropy) entropy[b] = m.bad ? quiet_nan() : q.live ? h : 0.0f;
-    if (row_state) row_state[b] = takes || m.bad ? 0.0f : -0.0f;
+    if (kLines) row_state[b] = takes || m.bad ? 0.0f : -0.0f;
   }
 }
 
 // 40 registers, 48 warps on an SM: with 48 registers 50021 bf16 positions took
 // 29 us instead of 25.
-__global__ void __launch_bounds__(32 * kMaxWarps, 6)
+constexpr int kScoreCtas = 6, kLineCtas = 4;
+template <bool kLines>
+__global__ void __launch_bounds__(32 * kMaxWarps, kLines ? kLineCtas : kScoreCtas)
     move_logprobs_kernel(const __grid_constant__ PolicyRows r, float *move_logp,
                          float *played_logp, float *entropy, float *row_state) {
   __shared__ Turns turns;
@@ -589,15 +614,14 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 6)
   pdl_wait();
   pdl_launch();
   const int lane = threadIdx.x & 31;
-  const float inv_temp2 = r.inv_temp * kLog2e;
   for_positions(
       r, gridDim.x, &turns,
       [&](int b, const Moves &m, int c0, int c1) {
-        score_position<2>(r, inv_temp2, b, m, c0, c1, lane, move_logp, played_logp, entropy, row_state);
+        score_position<2, kLines>(r, b, m, c0, c1, lane, move_logp, played_logp, entropy, row_state);
         return false;
       },
       [&](int b, const Moves &m) {
-        score_position<8>(r, inv_temp2, b, m, load_index(r, m, 0, lane), load_index(r, m, 1, lane),
+        score_position<8, kLines>(r, b, m, load_index(r, m, 0, lane), load_index(r, m, 1, lane),
                           lane, move_logp, played_logp, entropy, row_state);
       });
 }
@@ -621,7 +645,7 @@ struct BackArgs {
 
 template <int G>
 __device__ __forceinline__ void back_position(const PolicyRows &r, const BackArgs &a,
-                                              float inv_temp2, int b, const Moves &m, int c0,
+                                              int b, const Moves &m, int c0,
                                               int c1, int lane, RowImage &im) {
   Edges<G> v;
   columns<G>(r, m, c0, c1, lane, v);
@@ -638,7 +662,7 @@ __device__ __forceinline__ void back_position(const PolicyRows &r, const BackArg
   const float gh = a.entropy ? a.entropy[b] : 0.0f;
   logits_of<G>(m.n, row, r.type, v.col, bits, v.z);
   float es;
-  Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, inv_temp2, lane, v.e, es);
+  Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, lane, v.e, es);
   const float h = softmax_done<false>(q, es, q, total, lane);
 #pragma unroll
   for (int k = 0; k < G; ++k) {
@@ -717,18 +741,17 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3)
     sum_losses(a.loss, a.n, a.total, 1);
     return;
   }
-  const float inv_temp2 = r.inv_temp * kLog2e;
   for_positions(
       r, ctas, &turns,
       [&](int b, const Moves &m, int c0, int c1) {
-        back_position<2>(r, a, inv_temp2, b, m, c0, c1, lane, im);
+        back_position<2>(r, a, b, m, c0, c1, lane, im);
         return false;
       },
       [&](int b, const Moves &m) {
         if (m.bad)
           write_nan_row(a.out, r.classes, b, lane);
         else
-          back_position<8>(r, a, inv_temp2, b, m, load_index(r, m, 0, lane),
+          back_position<8>(r, a, b, m, load_index(r, m, 0, lane),
                            load_index(r, m, 1, lane), lane, im);
       });
   if (lane == 0) bulk_wait0();
@@ -766,7 +789,7 @@ __device__ __forceinline__ float kl_term(float p, float pr, float d) {
 // to be decided in 32 bits, unless kExact.
 template <int G, bool kExact>
 __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArgs &a,
-                                              float inv_temp2, int b, const Moves &m, int c0,
+                                              int b, const Moves &m, int c0,
                                               int c1, int lane, RowImage &im) {
   Edges<G> v;
   columns<G>(r, m, c0, c1, lane, v);
@@ -781,11 +804,11 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   logits_of<G>(m.n, row, r.type, v.col, bits, v.z);
   if (a.ref) logits_of<G>(m.n, ref, a.ref_type, v.col, ref_bits, d);
   float es;
-  Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, inv_temp2, lane, v.e, es);
+  Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, lane, v.e, es);
   float h, kl = 0.0f;
   if (a.ref) {
     float er[G], es_r;
-    Norm w = softmax_part<G>(m.n, d, r.inv_temp, inv_temp2, lane, er, es_r);
+    Norm w = softmax_part<G>(m.n, d, r.inv_temp, lane, er, es_r);
     h = softmax_done<true>(q, es, w, kl, lane);
 #pragma unroll
     for (int k = 0; k < G; ++k) {
@@ -802,7 +825,7 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   const bool takes = q.live && m.played >= 0;
   const float za = of_move<G>(v.z, m.played < 0 ? 0 : m.played, lane);
   const float sa = (za - q.top) * r.inv_temp;
-  const float ratio = exp2_fast(((sa - old) - q.log_s) * kLog2e);
+  const float ratio = exp_fast((sa - old) - q.log_s);
   // The gradient jumps where the ratio crosses the clip's border, so a ratio
   // within the rounding of the border is computed again in 64 bits.
   const float border = static_cast<float>(adv > 0.0f ? a.high : a.low);
@@ -863,15 +886,14 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3)
   start_turns(&turns);
   pdl_wait();
   pdl_launch();
-  const float inv_temp2 = r.inv_temp * kLog2e;
   for_positions(
       r, gridDim.x, &turns,
       [&](int b, const Moves &m, int c0, int c1) {
-        return clip_position<2, false>(r, a, inv_temp2, b, m, c0, c1, lane, im);
+        return clip_position<2, false>(r, a, b, m, c0, c1, lane, im);
       },
       [&](int b, const Moves &m) {
         if (!m.bad) {
-          clip_position<8, true>(r, a, inv_temp2, b, m, load_index(r, m, 0, lane),
+          clip_position<8, true>(r, a, b, m, load_index(r, m, 0, lane),
                                  load_index(r, m, 1, lane), lane, im);
           return;
         }
@@ -1030,9 +1052,9 @@ cudaError_t launch_total(const float *loss, int n, float *total, cudaStream_t s)
 
 cudaError_t launch_move_logprobs(const PolicyRows &r, float *move_logp, float *played_logp,
                                  float *entropy, float *row_state, cudaStream_t s) {
-  const Shape t = shape_for(r.batch, kMaxWarps, 6, 0);
-  return launch_k(move_logprobs_kernel, dim3(t.ctas), dim3(32 * t.warps), 0, s, 1, r, move_logp,
-                  played_logp, entropy, row_state);
+  const Shape t = shape_for(r.batch, kMaxWarps, row_state ? kLineCtas : kScoreCtas, 0);
+  return launch_k(row_state ? move_logprobs_kernel<true> : move_logprobs_kernel<false>, dim3(t.ctas),
+                  dim3(32 * t.warps), 0, s, 1, r, move_logp, played_logp, entropy, row_state);
 }
 
 }  // namespace mfb200
@@ -1132,6 +1154,7 @@ PolicyRows rows_of(const mfb200_policy_rows &r) {
   o.played = r.played;
   o.temp = r.softmax_temp;
   o.inv_temp = static_cast<float>(1.0 / r.softmax_temp);
+  o.inv_temp_rest = static_cast<float>(1.0 / r.softmax_temp - static_cast<double>(o.inv_temp));
   return o;
 }
 

@@ -18,7 +18,7 @@ struct PolicyRows {
   long long num_moves;
   const int32_t *played;  // [batch] edge numbers, or null
   double temp;
-  float inv_temp;
+  float inv_temp, inv_temp_rest;  // 1 / temp in two parts
 };
 
 // Log-probabilities of the legal moves, of the played move and the entropy;

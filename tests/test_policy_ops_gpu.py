@@ -310,6 +310,22 @@ def test_preference_loss(dtype, beta, eps, temp, shift, pad):
     check_preference(x, out, rows, logp, frozen, cuts, beta, eps, w, 8.0)
 
 
+def test_preference_margins_of_long_lines():
+    """What leans to one side in a log-probability adds up over the 400 positions
+    that one line is longer than the other. Each value: the exponentials 4 u
+    and their arguments u |s|, weighted by p at most 4 u + 6 u, seven additions
+    7 u, one rounding u |logp|. Their mean: errors of either sign, of 2 u (rms)
+    at most, leave 2 u / sqrt(1200) = 0.06 u; 0.3 u is five times that."""
+    temp = 1.93  # neither it nor its reciprocal is an fp32 number
+    x = Batch("f32", 1858, [int(n) for n in np.random.default_rng(5).integers(2, 60, 1200)], 29, temp)
+    rows, logp, frozen, lines = line_case(x, [0, 800, 1200])
+    out = policy.preference_loss(*x.args(), lines, x.f32(frozen), beta=0.1, softmax_temp=temp)
+    off = (out.logp.double().cpu().numpy() - logp) / ref.U
+    assert np.all(np.abs(off) <= 17 + np.abs(logp))
+    assert abs(off.mean()) <= 0.3
+    check_preference(x, out, rows, logp, frozen, [0, 800, 1200], 0.1, 0.0, [1.0], 1.0)
+
+
 @pytest.mark.parametrize("pairs,plies", [(1, 1), (300, 4), (2, 700), (1300, 1)])
 def test_preference_loss_sizes(pairs, plies):
     rng = np.random.default_rng(pairs)
@@ -399,6 +415,10 @@ def test_nan_and_infinity_among_listed_logits_stay_in_their_row():
     got = policy.clipped_policy_loss(*x.args(), zero - 3, one, entropy_coef=0.1)
     assert torch.isnan(got.loss).cpu().tolist() == bad
     assert torch.isnan(got.grad_logits).any(1).cpu().tolist() == bad
+    lines = torch.arange(9, dtype=torch.int32, device="cuda").clamp(max=4)
+    pref = policy.preference_loss(*x.args(), lines, zero - 3)
+    assert torch.isnan(pref.logp).cpu().tolist() == bad
+    assert torch.isnan(pref.margin).cpu().tolist() == [True, True, False, False]
     off = torch.ones(1858, dtype=torch.bool)
     off[torch.from_numpy(np.asarray(x.lists[1], np.int64))] = False
     assert (got.grad_logits[1].cpu()[off] == 0).all()
