@@ -106,7 +106,7 @@ def _lib():
 def _vector(t, name, dtype, size, device):
     """Pointer of a contiguous 1-D tensor of the given type and size (None: any)."""
     try:
-        if (t.dtype is dtype and t.dim() == 1 and t.get_device() == device and t.is_contiguous()
+        if (t.dtype is dtype and t.get_device() == device and t.is_contiguous() and t.dim() == 1
                 and (size is None or t.numel() == size)):
             return t.data_ptr()
     except AttributeError:
@@ -137,29 +137,33 @@ def _matrix(t, name, shape, device):
 
 
 def _rows(logits, move_offsets, move_index, played, softmax_temp):
-    """The C struct and the device's index."""
-    if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
+    """The C struct, the logits' shape and the device's index."""
+    kind = TYPES.get(logits.dtype) if isinstance(logits, torch.Tensor) else None
+    if kind is None or logits.dim() != 2:
         raise ValueError("logits must be a 2-D float32, bfloat16 or float16 tensor")
     device = logits.get_device()
     if device < 0:
         raise ValueError("logits must be a CUDA tensor: there is no CPU path")
     shape = logits.shape
     batch, classes = shape
-    ptr, stride, kind = _matrix(logits, "logits", shape, device)
+    stride, unit = logits.stride()
+    if unit != 1 and classes > 1:
+        raise ValueError("logits must have unit stride along a row")
     off = _vector(move_offsets, "move_offsets", torch.int32, batch + 1, device)
     index = _vector(move_index, "move_index", torch.int16, None, device)
     at = None if played is None else _vector(played, "played", torch.int32, batch, device)
-    return _Rows(ptr, stride, kind, batch, classes, off, index, move_index.numel(), at,
-                 softmax_temp), device
+    return _Rows(logits.data_ptr(), stride if batch > 1 else classes, kind, batch, classes, off,
+                 index, move_index.numel(), at, softmax_temp), shape, device
 
 
-def _gradient(logits, grad, grad_logits, device):
+def _gradient(logits, shape, grad, grad_logits, device):
     """(tensor, pointer, row stride, type) of the gradient to write."""
     if grad_logits is None:
         if not grad:
             return None, None, 0, 0
         grad_logits = torch.empty_like(logits)  # contiguous for rows that are padded
-    return (grad_logits, *_matrix(grad_logits, "grad_logits", logits.shape, device))
+        return grad_logits, grad_logits.data_ptr(), shape[1], TYPES[grad_logits.dtype]
+    return (grad_logits, *_matrix(grad_logits, "grad_logits", shape, device))
 
 
 def _call(fn, device, *args):
@@ -183,11 +187,11 @@ def move_logprobs(logits, move_offsets, move_index, played=None, *,
     """Log-probabilities of the legal moves, of the played moves and the
     entropy of each position (``mfb200_move_logprobs``)."""
     L = _lib()
-    rows, device = _rows(logits, move_offsets, move_index, played, softmax_temp)
+    rows, shape, device = _rows(logits, move_offsets, move_index, played, softmax_temp)
     f = torch.float32
     moves = torch.empty_like(move_index, dtype=f)
     at = None if played is None else torch.empty_like(played, dtype=f)
-    entropy = logits.new_empty(rows.batch, dtype=f)
+    entropy = logits.new_empty(shape[0], dtype=f) if at is None else torch.empty_like(at)
     _call(L.mfb200_move_logprobs, device, rows, moves.data_ptr(),
           None if at is None else at.data_ptr(), entropy.data_ptr())
     return MoveLogprobs(moves, at, entropy)
@@ -201,14 +205,14 @@ def move_logprobs_backward(logits, move_offsets, move_index, played=None, *, gra
     ``grad_moves = -target`` this is the gradient of the cross-entropy to a
     distribution over the legal moves, such as the search's visit counts."""
     L = _lib()
-    rows, device = _rows(logits, move_offsets, move_index, played, softmax_temp)
+    rows, shape, device = _rows(logits, move_offsets, move_index, played, softmax_temp)
     f = torch.float32
-    gm = None if grad_moves is None else _vector(grad_moves, "grad_moves", f, rows.num_moves, device)
-    gp = None if grad_played is None else _vector(grad_played, "grad_played", f, rows.batch, device)
-    gh = None if grad_entropy is None else _vector(grad_entropy, "grad_entropy", f, rows.batch, device)
+    gm = None if grad_moves is None else _vector(grad_moves, "grad_moves", f, move_index.numel(), device)
+    gp = None if grad_played is None else _vector(grad_played, "grad_played", f, shape[0], device)
+    gh = None if grad_entropy is None else _vector(grad_entropy, "grad_entropy", f, shape[0], device)
     if gp is not None and played is None:
         raise ValueError("grad_played needs played")
-    grad, ptr, stride, kind = _gradient(logits, True, grad_logits, device)
+    grad, ptr, stride, kind = _gradient(logits, shape, True, grad_logits, device)
     _call(L.mfb200_move_logprobs_backward, device, rows, gm, gp, gh, ptr, stride, kind)
     return grad
 
@@ -222,16 +226,16 @@ def clipped_policy_loss(logits, move_offsets, move_index, played, old_logp, adva
     gradient (``mfb200_clipped_policy_loss``). ``old_logp``, ``advantage`` and
     ``weight`` are float32 [batch]; ``scale`` defaults to 1 / batch."""
     L = _lib()
-    rows, device = _rows(logits, move_offsets, move_index, played, softmax_temp)
+    rows, shape, device = _rows(logits, move_offsets, move_index, played, softmax_temp)
     if played is None:
         raise ValueError("played must be a 1-D torch.int32 tensor")
-    n, f = rows.batch, torch.float32
+    n, f = shape[0], torch.float32
     old = _vector(old_logp, "old_logp", f, n, device)
     adv = _vector(advantage, "advantage", f, n, device)
     w = None if weight is None else _vector(weight, "weight", f, n, device)
     ref, ref_stride, ref_kind = ((None, 0, 0) if ref_logits is None
-                                 else _matrix(ref_logits, "ref_logits", logits.shape, device))
-    g, ptr, stride, kind = _gradient(logits, grad, grad_logits, device)
+                                 else _matrix(ref_logits, "ref_logits", shape, device))
+    g, ptr, stride, kind = _gradient(logits, shape, grad, grad_logits, device)
     cfg = _ClipConfig(clip_low, clip_high, kl_coef, entropy_coef,
                       scale if scale is not None else 1.0 / max(n, 1))
     total = old_logp.new_empty(())
@@ -254,17 +258,17 @@ def preference_loss(logits, move_offsets, move_index, played, line_offsets, ref_
     ``ref_logp`` float32 [batch] is the reference policy's log-probability of
     each played move, ``weight`` float32 [pairs]; ``scale`` defaults to 1 / pairs."""
     L = _lib()
-    rows, device = _rows(logits, move_offsets, move_index, played, softmax_temp)
+    rows, shape, device = _rows(logits, move_offsets, move_index, played, softmax_temp)
     if played is None:
         raise ValueError("played must be a 1-D torch.int32 tensor")
-    n, f = rows.batch, torch.float32
+    n, f = shape[0], torch.float32
     lines = _vector(line_offsets, "line_offsets", torch.int32, None, device)
     if line_offsets.numel() % 2 != 1:
         raise ValueError("line_offsets must have 2 * pairs + 1 entries")
     pairs = line_offsets.numel() // 2
     ref = _vector(ref_logp, "ref_logp", f, n, device)
     w = None if weight is None else _vector(weight, "weight", f, pairs, device)
-    g, ptr, stride, kind = _gradient(logits, grad, grad_logits, device)
+    g, ptr, stride, kind = _gradient(logits, shape, grad, grad_logits, device)
     cfg = _PreferenceConfig(beta, label_smoothing, scale if scale is not None else 1.0 / max(pairs, 1))
     total = ref_logp.new_empty(())
     logp, row_grad = torch.empty_like(ref_logp), torch.empty_like(ref_logp)
