@@ -31,6 +31,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstdio>
+#include <type_traits>
 
 #include "../../include/mfb200.h"
 #include "gemm_host.h"  // num_sms
@@ -73,6 +74,16 @@ __device__ __forceinline__ float value_of(int type, unsigned bits) {
   return type == MFB200_TYPE_F32    ? __uint_as_float(bits)
          : type == MFB200_TYPE_BF16 ? __uint_as_float(bits << 16)
                                     : __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+}
+
+// The types of a call's matrices are template arguments where they are the same,
+// and looked at for every value (kAnyType) where they differ: 16384 bf16
+// positions' scores and gradient take 31 us instead of 33, 96 pairs of games 47
+// instead of 50.
+constexpr int kAnyType = -1;
+template <int kType>
+__device__ __forceinline__ int type_of(int type) {
+  return kType == kAnyType ? type : kType;
 }
 
 __device__ __forceinline__ const void *row_of(const void *base, int type, long long stride, int b) {
@@ -460,10 +471,10 @@ __device__ __forceinline__ void take_out(RowImage &im, int size, int lane) {
 // Writes row b: g[k] at the columns of the list, 0 elsewhere. A column that is
 // listed more than once gets the sum of its values, in the list's order; the
 // moves find that out by leaving their numbers in the image.
-template <int G>
+template <int G, int kType>
 __device__ __forceinline__ void write_row(RowImage &im, const Grad &out, int classes, int b, int n,
                                           int lane, const int (&col)[G], float (&g)[G]) {
-  const int size = out.type == MFB200_TYPE_F32 ? 4 : 2;
+  const int type = type_of<kType>(out.type), size = type == MFB200_TYPE_F32 ? 4 : 2;
   char *dst = static_cast<char *>(out.base) + b * out.stride * size;
   const int shift = static_cast<int>(reinterpret_cast<unsigned long long>(dst) & 15);
   int at[G];
@@ -509,7 +520,7 @@ __device__ __forceinline__ void write_row(RowImage &im, const Grad &out, int cla
   __syncwarp();
 #pragma unroll
   for (int k = 0; k < G; ++k)
-    if (32 * k < n && at[k] >= 0) put(im.buf + at[k], size, bits_of(out.type, g[k]));
+    if (32 * k < n && at[k] >= 0) put(im.buf + at[k], size, bits_of(type, g[k]));
   fence_proxy_async_smem();
   __syncwarp();
   // [shift, end) of the image is the row; [lo, hi) of it lies between 16-byte boundaries
@@ -555,7 +566,7 @@ __device__ __forceinline__ void write_nan_row(const Grad &out, int classes, int 
 // exponential and the rounding of 1 / T do, by some 1e-8): it is made from the
 // accurate exponential, 1 / T in two parts and a 64-bit logarithm, and rounded
 // once. row_state is then set.
-template <int G, bool kLines>
+template <int G, bool kLines, int kType>
 __device__ __forceinline__ void score_position(const PolicyRows &r, int b,
                                                const Moves &m, int c0, int c1, int lane,
                                                float *move_logp, float *played_logp,
@@ -563,9 +574,10 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, int b,
   Edges<G> v;
   columns<G>(r, m, c0, c1, lane, v);
   unsigned bits[G];
-  const void *row = row_of(r.logits, r.type, r.stride, b);
-  load_logits<G>(m.n, row, r.type, v.col, bits);
-  logits_of<G>(m.n, row, r.type, v.col, bits, v.z);
+  const int type = type_of<kType>(r.type);
+  const void *row = row_of(r.logits, type, r.stride, b);
+  load_logits<G>(m.n, row, type, v.col, bits);
+  logits_of<G>(m.n, row, type, v.col, bits, v.z);
   float es;
   Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, lane, v.e, es);
   float none = 0.0f;
@@ -605,7 +617,7 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, int b,
 // 40 registers, 48 warps on an SM: with 48 registers 50021 bf16 positions took
 // 29 us instead of 25.
 constexpr int kScoreCtas = 6, kLineCtas = 4;
-template <bool kLines>
+template <bool kLines, int kType>
 __global__ void __launch_bounds__(32 * kMaxWarps, kLines ? kLineCtas : kScoreCtas)
     move_logprobs_kernel(const __grid_constant__ PolicyRows r, float *move_logp,
                          float *played_logp, float *entropy, float *row_state) {
@@ -617,12 +629,14 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kLines ? kLineCtas : kScoreCta
   for_positions(
       r, gridDim.x, &turns,
       [&](int b, const Moves &m, int c0, int c1) {
-        score_position<2, kLines>(r, b, m, c0, c1, lane, move_logp, played_logp, entropy, row_state);
+        score_position<2, kLines, kType>(r, b, m, c0, c1, lane, move_logp, played_logp, entropy,
+                                         row_state);
         return false;
       },
       [&](int b, const Moves &m) {
-        score_position<8, kLines>(r, b, m, load_index(r, m, 0, lane), load_index(r, m, 1, lane),
-                          lane, move_logp, played_logp, entropy, row_state);
+        score_position<8, kLines, kType>(r, b, m, load_index(r, m, 0, lane),
+                                         load_index(r, m, 1, lane), lane, move_logp, played_logp,
+                                         entropy, row_state);
       });
 }
 
@@ -643,15 +657,16 @@ struct BackArgs {
   float *total;
 };
 
-template <int G>
+template <int G, int kType>
 __device__ __forceinline__ void back_position(const PolicyRows &r, const BackArgs &a,
                                               int b, const Moves &m, int c0,
                                               int c1, int lane, RowImage &im) {
   Edges<G> v;
   columns<G>(r, m, c0, c1, lane, v);
   unsigned bits[G];
-  const void *row = row_of(r.logits, r.type, r.stride, b);
-  load_logits<G>(m.n, row, r.type, v.col, bits);
+  const int type = type_of<kType>(r.type);
+  const void *row = row_of(r.logits, type, r.stride, b);
+  load_logits<G>(m.n, row, type, v.col, bits);
   float g[G], total = 0.0f;
 #pragma unroll
   for (int k = 0; k < G; ++k) {
@@ -660,7 +675,7 @@ __device__ __forceinline__ void back_position(const PolicyRows &r, const BackArg
   }
   const float ga = a.played && m.played >= 0 ? a.played[b] : 0.0f;
   const float gh = a.entropy ? a.entropy[b] : 0.0f;
-  logits_of<G>(m.n, row, r.type, v.col, bits, v.z);
+  logits_of<G>(m.n, row, type, v.col, bits, v.z);
   float es;
   Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, lane, v.e, es);
   const float h = softmax_done<false>(q, es, q, total, lane);
@@ -674,7 +689,7 @@ __device__ __forceinline__ void back_position(const PolicyRows &r, const BackArg
     g[k] = t * r.inv_temp;
     if (!q.live) v.col[k] = kNoColumn;
   }
-  write_row<G>(im, a.out, r.classes, b, m.n, lane, v.col, g);
+  write_row<G, kType>(im, a.out, r.classes, b, m.n, lane, v.col, g);
 }
 
 // The sum of n losses by the `ctas` CTAs of a cluster (or one CTA), in 64 bits
@@ -725,12 +740,13 @@ __device__ void sum_losses(const float *loss, int n, float *total, unsigned ctas
   cluster_sync();  // no CTA leaves while its part is read
 }
 
+template <int kType>
 __global__ void __launch_bounds__(32 * kMaxWarps, 3)
     move_logprobs_backward_kernel(const __grid_constant__ PolicyRows r,
                                   const __grid_constant__ BackArgs a) {
   extern __shared__ __align__(16) char images[];
   const int lane = threadIdx.x & 31;
-  const int row_bytes = r.classes * (a.out.type == MFB200_TYPE_F32 ? 4 : 2);
+  const int row_bytes = r.classes * (type_of<kType>(a.out.type) == MFB200_TYPE_F32 ? 4 : 2);
   const unsigned ctas = gridDim.x - (a.total ? 1 : 0);
   RowImage im = clear_image(images + (threadIdx.x >> 5) * image_bytes(row_bytes), row_bytes, lane);
   __shared__ Turns turns;
@@ -744,15 +760,15 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3)
   for_positions(
       r, ctas, &turns,
       [&](int b, const Moves &m, int c0, int c1) {
-        back_position<2>(r, a, b, m, c0, c1, lane, im);
+        back_position<2, kType>(r, a, b, m, c0, c1, lane, im);
         return false;
       },
       [&](int b, const Moves &m) {
         if (m.bad)
           write_nan_row(a.out, r.classes, b, lane);
         else
-          back_position<8>(r, a, b, m, load_index(r, m, 0, lane),
-                           load_index(r, m, 1, lane), lane, im);
+          back_position<8, kType>(r, a, b, m, load_index(r, m, 0, lane),
+                                  load_index(r, m, 1, lane), lane, im);
       });
   if (lane == 0) bulk_wait0();
 }
@@ -787,7 +803,7 @@ __device__ __forceinline__ float kl_term(float p, float pr, float d) {
 
 // Returns true, with nothing written, for a ratio too near the clip's border
 // to be decided in 32 bits, unless kExact.
-template <int G, bool kExact>
+template <int G, bool kExact, int kType>
 __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArgs &a,
                                               int b, const Moves &m, int c0,
                                               int c1, int lane, RowImage &im) {
@@ -795,14 +811,16 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   columns<G>(r, m, c0, c1, lane, v);
   float d[G];  // the reference's logits, then d = log p - log q
   unsigned bits[G], ref_bits[G];
-  const void *row = row_of(r.logits, r.type, r.stride, b);
-  load_logits<G>(m.n, row, r.type, v.col, bits);
-  const void *ref = a.ref ? row_of(a.ref, a.ref_type, a.ref_stride, b) : nullptr;
-  if (a.ref) load_logits<G>(m.n, ref, a.ref_type, v.col, ref_bits);
+  const int type = type_of<kType>(r.type);
+  const void *row = row_of(r.logits, type, r.stride, b);
+  load_logits<G>(m.n, row, type, v.col, bits);
+  const int ref_type = type_of<kType>(a.ref_type);
+  const void *ref = a.ref ? row_of(a.ref, ref_type, a.ref_stride, b) : nullptr;
+  if (a.ref) load_logits<G>(m.n, ref, ref_type, v.col, ref_bits);
   const float old = a.old_logp[b], adv = a.advantage[b];
   const float c = a.scale * (a.weight ? a.weight[b] : 1.0f);
-  logits_of<G>(m.n, row, r.type, v.col, bits, v.z);
-  if (a.ref) logits_of<G>(m.n, ref, a.ref_type, v.col, ref_bits, d);
+  logits_of<G>(m.n, row, type, v.col, bits, v.z);
+  if (a.ref) logits_of<G>(m.n, ref, ref_type, v.col, ref_bits, d);
   float es;
   Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, lane, v.e, es);
   float h, kl = 0.0f;
@@ -857,7 +875,7 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
       g[k] = c * r.inv_temp * t;
       if (!takes) v.col[k] = kNoColumn;
     }
-    write_row<G>(im, a.grad, r.classes, b, m.n, lane, v.col, g);
+    write_row<G, kType>(im, a.grad, r.classes, b, m.n, lane, v.col, g);
   }
   // after the row: the fence before its copy would wait for these stores
   if (lane == 0) {
@@ -872,6 +890,7 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   return false;
 }
 
+template <int kType>
 __global__ void __launch_bounds__(32 * kMaxWarps, 3)
     clipped_policy_loss_kernel(const __grid_constant__ PolicyRows r,
                                const __grid_constant__ ClipArgs a) {
@@ -879,7 +898,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3)
   const int lane = threadIdx.x & 31;
   RowImage im{};
   if (a.grad.base) {
-    const int row_bytes = r.classes * (a.grad.type == MFB200_TYPE_F32 ? 4 : 2);
+    const int row_bytes = r.classes * (type_of<kType>(a.grad.type) == MFB200_TYPE_F32 ? 4 : 2);
     im = clear_image(images + (threadIdx.x >> 5) * image_bytes(row_bytes), row_bytes, lane);
   }
   __shared__ Turns turns;
@@ -889,12 +908,12 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3)
   for_positions(
       r, gridDim.x, &turns,
       [&](int b, const Moves &m, int c0, int c1) {
-        return clip_position<2, false>(r, a, b, m, c0, c1, lane, im);
+        return clip_position<2, false, kType>(r, a, b, m, c0, c1, lane, im);
       },
       [&](int b, const Moves &m) {
         if (!m.bad) {
-          clip_position<8, true>(r, a, b, m, load_index(r, m, 0, lane),
-                                 load_index(r, m, 1, lane), lane, im);
+          clip_position<8, true, kType>(r, a, b, m, load_index(r, m, 0, lane),
+                                        load_index(r, m, 1, lane), lane, im);
           return;
         }
         if (lane == 0) {
@@ -1016,19 +1035,38 @@ cudaError_t allow_images(K *kernel, std::atomic<unsigned long long> &done) {
   return e;
 }
 
+// launch(type) with the type as a constant.
+template <class Launch>
+cudaError_t with_type(int type, Launch launch) {
+  switch (type) {
+    case MFB200_TYPE_F32: return launch(std::integral_constant<int, MFB200_TYPE_F32>());
+    case MFB200_TYPE_BF16: return launch(std::integral_constant<int, MFB200_TYPE_BF16>());
+    default: return launch(std::integral_constant<int, MFB200_TYPE_F16>());
+  }
+}
+
 cudaError_t launch_backward(const PolicyRows &r, const BackArgs &a, cudaStream_t s) {
-  static std::atomic<unsigned long long> done{0};
-  if (cudaError_t e = allow_images(move_logprobs_backward_kernel, done)) return e;
   const Shape t = shape_with_images(r, a.out);
-  return launch_k(move_logprobs_backward_kernel, dim3(t.ctas + (a.total ? 1 : 0)),
-                  dim3(32 * t.warps), t.smem, s, 1, r, a);
+  const auto launch = [&](auto type) {
+    static std::atomic<unsigned long long> done{0};
+    constexpr auto *kernel = move_logprobs_backward_kernel<decltype(type)::value>;
+    if (cudaError_t e = allow_images(kernel, done)) return e;
+    return launch_k(kernel, dim3(t.ctas + (a.total ? 1 : 0)), dim3(32 * t.warps), t.smem, s, 1, r, a);
+  };
+  return a.out.type == r.type ? with_type(r.type, launch)
+                              : launch(std::integral_constant<int, kAnyType>());
 }
 
 cudaError_t launch_clip(const PolicyRows &r, const ClipArgs &a, cudaStream_t s) {
-  static std::atomic<unsigned long long> done{0};
-  if (cudaError_t e = allow_images(clipped_policy_loss_kernel, done)) return e;
   const Shape t = a.grad.base ? shape_with_images(r, a.grad) : shape_for(r.batch, kMaxWarps, 3, 0);
-  return launch_k(clipped_policy_loss_kernel, dim3(t.ctas), dim3(32 * t.warps), t.smem, s, 1, r, a);
+  const bool same = (!a.ref || a.ref_type == r.type) && (!a.grad.base || a.grad.type == r.type);
+  const auto launch = [&](auto type) {
+    static std::atomic<unsigned long long> done{0};
+    constexpr auto *kernel = clipped_policy_loss_kernel<decltype(type)::value>;
+    if (cudaError_t e = allow_images(kernel, done)) return e;
+    return launch_k(kernel, dim3(t.ctas), dim3(32 * t.warps), t.smem, s, 1, r, a);
+  };
+  return same ? with_type(r.type, launch) : launch(std::integral_constant<int, kAnyType>());
 }
 
 cudaError_t launch_pairs(int pairs, int batch, const int32_t *lines, const float *logp,
@@ -1053,8 +1091,12 @@ cudaError_t launch_total(const float *loss, int n, float *total, cudaStream_t s)
 cudaError_t launch_move_logprobs(const PolicyRows &r, float *move_logp, float *played_logp,
                                  float *entropy, float *row_state, cudaStream_t s) {
   const Shape t = shape_for(r.batch, kMaxWarps, row_state ? kLineCtas : kScoreCtas, 0);
-  return launch_k(row_state ? move_logprobs_kernel<true> : move_logprobs_kernel<false>, dim3(t.ctas),
-                  dim3(32 * t.warps), 0, s, 1, r, move_logp, played_logp, entropy, row_state);
+  return with_type(r.type, [&](auto type) {
+    constexpr int kType = decltype(type)::value;
+    return launch_k(row_state ? move_logprobs_kernel<true, kType> : move_logprobs_kernel<false, kType>,
+                    dim3(t.ctas), dim3(32 * t.warps), 0, s, 1, r, move_logp, played_logp, entropy,
+                    row_state);
+  });
 }
 
 }  // namespace mfb200
