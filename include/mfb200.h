@@ -317,8 +317,10 @@ MFB200_API const char *mfb200_noalloc_last_error(void);
  * synchronising. The calls allocate nothing, keep nothing between calls and
  * can be captured into a CUDA graph (make a first call on the device before); calls on different streams or threads do
  * not share anything but the buffers they are given. Results do not depend on
- * timing: the same inputs give the same bits. Outputs may not overlap inputs or
- * one another. Returns 0 on success;
+ * timing: the same inputs give the same bits. (The one exception: offsets that
+ * decrease may put an entry of move_index into two lists, or a position into
+ * the lines of two pairs; its move_logp entry or its gradient is then either
+ * one's.) Outputs may not overlap inputs or one another. Returns 0 on success;
  * mfb200_policy_last_error() gives the calling thread's last message.
  *
  * The softmax of a position runs over its first n = min(count, 256) listed

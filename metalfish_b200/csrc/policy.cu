@@ -565,12 +565,13 @@ __device__ __forceinline__ void write_nan_row(const Grad &out, int classes, int 
 // differences are small, where what leans to one side adds up (the fast
 // exponential and the rounding of 1 / T do, by some 1e-8): it is made from the
 // accurate exponential, 1 / T in two parts and a 64-bit logarithm, and rounded
-// once. row_state is then set.
+// once. Its sign bit then tells whether the position takes part (set, for a NaN as
+// well) or has no move (+0), and row_grad gets the zero of a position in no line.
 template <int G, bool kLines, int kType>
 __device__ __forceinline__ void score_position(const PolicyRows &r, int b,
                                                const Moves &m, int c0, int c1, int lane,
                                                float *move_logp, float *played_logp,
-                                               float *entropy, float *row_state) {
+                                               float *entropy, float *row_grad) {
   Edges<G> v;
   columns<G>(r, m, c0, c1, lane, v);
   unsigned bits[G];
@@ -608,9 +609,14 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, int b,
       logp = static_cast<float>((static_cast<double>(z) - q.top) / r.temp - log(1.0 + rest));
   }
   if (lane == 0) {
-    if (played_logp) played_logp[b] = m.bad ? quiet_nan() : takes ? logp : 0.0f;
+    const float value = m.bad ? quiet_nan() : takes ? logp : 0.0f;
+    // (a log-probability is never above 0)
+    if (kLines)
+      played_logp[b] = takes || m.bad ? __uint_as_float(__float_as_uint(value) | 0x80000000u) : 0.0f;
+    else if (played_logp)
+      played_logp[b] = value;
     if (entropy) entropy[b] = m.bad ? quiet_nan() : q.live ? h : 0.0f;
-    if (kLines) row_state[b] = takes || m.bad ? 0.0f : -0.0f;
+    if (kLines) row_grad[b] = 0.0f;
   }
 }
 
@@ -620,7 +626,7 @@ constexpr int kScoreCtas = 6, kLineCtas = 4;
 template <bool kLines, int kType>
 __global__ void __launch_bounds__(32 * kMaxWarps, kLines ? kLineCtas : kScoreCtas)
     move_logprobs_kernel(const __grid_constant__ PolicyRows r, float *move_logp,
-                         float *played_logp, float *entropy, float *row_state) {
+                         float *played_logp, float *entropy, float *row_grad) {
   __shared__ Turns turns;
   start_turns(&turns);
   pdl_wait();
@@ -630,13 +636,13 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kLines ? kLineCtas : kScoreCta
       r, gridDim.x, &turns,
       [&](int b, const Moves &m, int c0, int c1) {
         score_position<2, kLines, kType>(r, b, m, c0, c1, lane, move_logp, played_logp, entropy,
-                                         row_state);
+                                         row_grad);
         return false;
       },
       [&](int b, const Moves &m) {
         score_position<8, kLines, kType>(r, b, m, load_index(r, m, 0, lane),
                                          load_index(r, m, 1, lane), lane, move_logp, played_logp,
-                                         entropy, row_state);
+                                         entropy, row_grad);
       });
 }
 
@@ -931,9 +937,9 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3)
 // One warp per pair of lines. With D = the sum over a line's rows of
 // (logp - ref) and m = beta (D_preferred - D_rejected):
 //     L = scale w ( -(1 - eps) log sigma(m) - eps log sigma(-m) ),
-// and dL/dlogp of a row is +-beta dL/dm, written over the row's state (+0: the
-// row takes part; -0: it does not, its reference value is left out). Rows in no
-// line keep a zero. The sums run in 64 bits, in an order fixed by the rows.
+// and dL/dlogp of a row is +-beta dL/dm. A row whose logp has no sign bit takes no
+// part: its reference value is left out and its gradient zero. Rows in no line
+// keep the zero they have. The sums run in 64 bits, in an order fixed by the rows.
 __global__ void __launch_bounds__(256)
     preference_pair_kernel(int pairs, int batch, const int32_t *lines,
                            const float *logp, const float *ref,
@@ -958,9 +964,9 @@ __global__ void __launch_bounds__(256)
   for (int side = 0; side < 2; ++side) {
 #pragma unroll 4
     for (int b = at[side] + lane; b < at[side + 1]; b += 32) {
-      const float state = row_grad[b], lp = logp[b], frozen = ref[b];
-      sum[side] += signbit(state) ? 0.0 : static_cast<double>(lp);
-      gain[side] += signbit(state) ? 0.0 : static_cast<double>(lp) - static_cast<double>(frozen);
+      const float lp = logp[b], frozen = ref[b];
+      sum[side] += static_cast<double>(lp);
+      gain[side] += signbit(lp) ? static_cast<double>(lp) - static_cast<double>(frozen) : 0.0;
     }
     sum[side] = warp_sum(sum[side]);
     gain[side] = warp_sum(gain[side]);
@@ -983,7 +989,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int side = 0; side < 2; ++side)
     for (int b = at[side] + lane; b < at[side + 1]; b += 32)
-      row_grad[b] = signbit(row_grad[b]) ? 0.0f : side ? -slope : slope;
+      row_grad[b] = !signbit(logp[b]) ? 0.0f : side ? -slope : slope;
 }
 
 // ------------------------------------------------------------------ total
@@ -1089,13 +1095,13 @@ cudaError_t launch_total(const float *loss, int n, float *total, cudaStream_t s)
 }  // namespace
 
 cudaError_t launch_move_logprobs(const PolicyRows &r, float *move_logp, float *played_logp,
-                                 float *entropy, float *row_state, cudaStream_t s) {
-  const Shape t = shape_for(r.batch, kMaxWarps, row_state ? kLineCtas : kScoreCtas, 0);
+                                 float *entropy, float *row_grad, cudaStream_t s) {
+  const Shape t = shape_for(r.batch, kMaxWarps, row_grad ? kLineCtas : kScoreCtas, 0);
   return with_type(r.type, [&](auto type) {
     constexpr int kType = decltype(type)::value;
-    return launch_k(row_state ? move_logprobs_kernel<true, kType> : move_logprobs_kernel<false, kType>,
+    return launch_k(row_grad ? move_logprobs_kernel<true, kType> : move_logprobs_kernel<false, kType>,
                     dim3(t.ctas), dim3(32 * t.warps), 0, s, 1, r, move_logp, played_logp, entropy,
-                    row_state);
+                    row_grad);
   });
 }
 

@@ -22,9 +22,10 @@ struct PolicyRows {
 };
 
 // Log-probabilities of the legal moves, of the played move and the entropy;
-// each output may be null. row_state, if set, receives +0 for rows that take
-// part in a loss and -0 for rows that do not (see preference_pair_kernel).
+// each output may be null. With row_grad the played moves' log-probabilities are
+// made for sums over long lines, their signs tell which positions take part, and
+// row_grad is set to zero (see score_position and preference_pair_kernel).
 cudaError_t launch_move_logprobs(const PolicyRows &r, float *move_logp, float *played_logp,
-                                 float *entropy, float *row_state, cudaStream_t s);
+                                 float *entropy, float *row_grad, cudaStream_t s);
 
 }  // namespace mfb200

@@ -489,6 +489,22 @@ def test_malformed_lines_are_nan(cuts):
     assert torch.isfinite(out.grad_logits).all()
 
 
+def test_lines_that_two_pairs_share():
+    """Offsets that decrease between two pairs put positions into both: each
+    pair's results are those of its own lines, whichever is worked on first."""
+    x = Batch("f32", 1858, [20, 25, 0, 30], 18)
+    frozen = torch.tensor([-3.0, -2.0, -5.0, -1.0], device="cuda")
+    cuts = [0, 1, 4, 2, 1, 2, 4]  # (0, 1, 4) and (1, 2, 4) are in order, (4, 2, 1) is not
+    out = policy.preference_loss(*x.args(), torch.tensor(cuts, dtype=torch.int32, device="cuda"), frozen)
+    assert torch.isnan(out.loss).cpu().tolist() == [False, True, False]
+    for i in (0, 2):
+        own = torch.tensor(cuts[2 * i:2 * i + 3], dtype=torch.int32, device="cuda")
+        one = policy.preference_loss(*x.args(), own, frozen)
+        assert torch.equal(one.margin[0], out.margin[i])
+        assert torch.equal(one.line_logp, out.line_logp[2 * i:2 * i + 2])
+    assert torch.isfinite(out.grad_logits).all() and out.row_grad[2].item() == 0
+
+
 def test_nothing_at_all():
     off = torch.zeros(1, dtype=torch.int32, device="cuda")
     idx, none = torch.zeros(0, dtype=torch.int16, device="cuda"), torch.zeros(0, device="cuda")
