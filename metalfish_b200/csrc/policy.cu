@@ -115,7 +115,7 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 __device__ __forceinline__ float exp2_fast(float t) {
   float v;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(v) : "f"(t));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"(t));
   return v;
 }
 // e^s for s <= 0 as 2^(s log2 e), log2 e in two parts: the rounding of the
@@ -319,7 +319,7 @@ __device__ __forceinline__ void logits_of(int n, const void *row, int type, cons
 // so that log S and 1 - p of a nearly certain move keep their digits.
 struct Norm {
   float top;   // largest logit
-  int lead;    // lowest edge that has it
+  int lead;    // its edge in the lane that has it (the first such lane), else -1
   bool live;   // some move has a logit above -inf (or NaN)
   float rest;  // sum of exp(s - s_top) over the other moves
   float log_s, inv_s;
@@ -344,27 +344,33 @@ __device__ __forceinline__ Norm softmax_part(int n, const float (&z)[G], float i
     for (int k = 0; k < G; ++k) nan |= 32 * k < n && z[k] != z[k];
     q.live = __any_sync(kFull, nan);
   }
-  q.lead = -1;
   q.rest = 0.0f;
   es = 0.0f;
+  int mine = -1;  // this lane's lowest edge with the largest logit
 #pragma unroll
   for (int k = 0; k < G; ++k) {
     e[k] = 0.0f;
     if (32 * k < n) {
-      const unsigned at = __ballot_sync(kFull, z[k] == q.top);
-      if (q.lead < 0 && at) q.lead = 32 * k + __ffs(at) - 1;
       const float t = (z[k] - q.top) * inv_temp;
       e[k] = exp_fast(t);
       if (e[k] != 0.0f) es += e[k] * t;
-      if (32 * k + lane != q.lead) q.rest += e[k];
+      if (mine < 0 && z[k] == q.top)
+        mine = 32 * k + lane;
+      else
+        q.rest += e[k];
     }
   }
+  // every lane but the first that has one puts it back into the sum
+  const unsigned at = __ballot_sync(kFull, mine >= 0);
+  const int first = __ffs(at) - 1;
+  if (mine >= 0 && lane != first) q.rest += 1.0f;
+  q.lead = lane == first ? mine : -1;
   return q;
 }
 
 __device__ __forceinline__ float reciprocal(float x) {
   float v;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(v) : "f"(x));  // within one step
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"(x));  // within one step
   return v;
 }
 
@@ -620,9 +626,11 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, int b,
   }
 }
 
-// 40 registers, 48 warps on an SM: with 48 registers 50021 bf16 positions took
-// 29 us instead of 25.
-constexpr int kScoreCtas = 6, kLineCtas = 4;
+// CTAs on an SM. 40 warps with 48 registers: 50021 bf16 positions take 22 us; with
+// 48 warps and 40 registers 23, with 32 warps and 64 registers 27. For lines, whose
+// 64-bit logarithm wants more registers, 4 and 5 are alike (96 pairs of games 44 and
+// 46 us, 256 pairs of short lines 20 and 19).
+constexpr int kScoreCtas = 5, kLineCtas = 4;
 template <bool kLines, int kType>
 __global__ void __launch_bounds__(32 * kMaxWarps, kLines ? kLineCtas : kScoreCtas)
     move_logprobs_kernel(const __grid_constant__ PolicyRows r, float *move_logp,
