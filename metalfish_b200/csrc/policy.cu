@@ -374,37 +374,43 @@ __device__ __forceinline__ float reciprocal(float x) {
   return v;
 }
 
-// Ends softmax_part for a row and, with kSecond, for a second softmax w over
-// the same list: the sums over the warp, their logarithms and reciprocals.
-// Returns the entropy -sum p log p = log S - sum(e s) / S, two terms that are
-// never negative; without a second softmax `more` is summed as well.
+// Ends softmax_part for a row: the sums over the warp, their logarithm and
+// reciprocal. Returns the entropy -sum p log p = log S - sum(e s) / S, two terms
+// that are never negative. With kMore `more` is summed as well, with kSecond the
+// sum of a second softmax w over the same list.
 //
-// The three sums share one reduction: after the step over 16 lanes the lower
-// half works on one value and the upper on another, after the step over 8 each
-// quarter on one, so they take 6 shuffles instead of 15, and one logarithm and
-// one reciprocal serve both softmaxes.
-template <bool kSecond>
+// The sums share one reduction: after the step over 16 lanes the lower half works
+// on one value and the upper on another, after the step over 8 each quarter on
+// one, so three take 6 shuffles instead of 15 and two 5 instead of 10, and one
+// logarithm and one reciprocal serve both softmaxes.
+enum class Sums { kTwo, kMore, kSecond };
+template <Sums kSums>
 __device__ __forceinline__ float softmax_done(Norm &q, float es, Norm &w, float &more, int lane) {
+  constexpr bool kTwo = kSums == Sums::kTwo, kSecond = kSums == Sums::kSecond;
   const bool upper = lane & 16, second = lane & 8;
   if (q.top == INFINITY) q.rest = quiet_nan();  // its own inf - inf is not in the sum
   if (kSecond && w.top == INFINITY) w.rest = quiet_nan();
-  const float x = kSecond ? w.rest : more;
-  float a = (upper ? x : q.rest) + __shfl_xor_sync(kFull, upper ? q.rest : x, 16);
-  float b = es + __shfl_xor_sync(kFull, es, 16);
-  float v = (second ? b : a) + __shfl_xor_sync(kFull, second ? a : b, 8);
+  const float x = kTwo ? es : kSecond ? w.rest : more;
+  float v = (upper ? x : q.rest) + __shfl_xor_sync(kFull, upper ? q.rest : x, 16);
+  if (kTwo) {
+    v += __shfl_xor_sync(kFull, v, 8);
+  } else {
+    const float b = es + __shfl_xor_sync(kFull, es, 16);
+    v = (second ? b : v) + __shfl_xor_sync(kFull, second ? v : b, 8);
+  }
   v += __shfl_xor_sync(kFull, v, 4);
   v += __shfl_xor_sync(kFull, v, 2);
   v += __shfl_xor_sync(kFull, v, 1);
-  // lanes 0-7 hold q.rest, 16-23 w.rest or `more`, the others es
+  // lanes 0-7 hold q.rest, 16-23 es of two sums, w.rest or `more`, 8-15 es of three
   const float log_v = log1pf(v), inv_v = reciprocal(1.0f + v);
   q.rest = __shfl_sync(kFull, v, 0);
   q.log_s = __shfl_sync(kFull, log_v, 0);
   q.inv_s = __shfl_sync(kFull, inv_v, 0);
-  es = __shfl_sync(kFull, v, 8);
+  es = __shfl_sync(kFull, v, kTwo ? 16 : 8);
   if (kSecond) {
     w.log_s = __shfl_sync(kFull, log_v, 16);
     w.inv_s = __shfl_sync(kFull, inv_v, 16);
-  } else {
+  } else if (!kTwo) {
     more = __shfl_sync(kFull, v, 16);
   }
   return q.log_s - es * q.inv_s;
@@ -587,8 +593,7 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, int b,
   logits_of<G>(m.n, row, type, v.col, bits, v.z);
   float es;
   Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, lane, v.e, es);
-  float none = 0.0f;
-  const float h = softmax_done<false>(q, es, q, none, lane);
+  const float h = softmax_done<Sums::kTwo>(q, es, q, es, lane);
   if (move_logp) {
 #pragma unroll
     for (int k = 0; k < G; ++k) {
@@ -626,8 +631,8 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, int b,
   }
 }
 
-// CTAs on an SM. 40 warps with 48 registers: 50021 bf16 positions take 22 us; with
-// 48 warps and 40 registers 23, with 32 warps and 64 registers 27. For lines, whose
+// CTAs on an SM. 40 warps with 48 registers: 50021 bf16 positions take 21 us; with
+// 48 warps and 40 registers 22, with 32 warps and 64 registers 27. For lines, whose
 // 64-bit logarithm wants more registers, 4 and 5 are alike (96 pairs of games 44 and
 // 46 us, 256 pairs of short lines 20 and 19).
 constexpr int kScoreCtas = 5, kLineCtas = 4;
@@ -692,7 +697,7 @@ __device__ __forceinline__ void back_position(const PolicyRows &r, const BackArg
   logits_of<G>(m.n, row, type, v.col, bits, v.z);
   float es;
   Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, lane, v.e, es);
-  const float h = softmax_done<false>(q, es, q, total, lane);
+  const float h = softmax_done<Sums::kMore>(q, es, q, total, lane);
 #pragma unroll
   for (int k = 0; k < G; ++k) {
     if (32 * k >= m.n) continue;
@@ -841,7 +846,7 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   if (a.ref) {
     float er[G], es_r;
     Norm w = softmax_part<G>(m.n, d, r.inv_temp, lane, er, es_r);
-    h = softmax_done<true>(q, es, w, kl, lane);
+    h = softmax_done<Sums::kSecond>(q, es, w, kl, lane);
 #pragma unroll
     for (int k = 0; k < G; ++k) {
       if (32 * k < m.n) {
@@ -852,7 +857,7 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
     }
     kl = warp_sum(kl);
   } else {
-    h = softmax_done<false>(q, es, q, kl, lane);
+    h = softmax_done<Sums::kTwo>(q, es, q, kl, lane);
   }
   const bool takes = q.live && m.played >= 0;
   const float za = of_move<G>(v.z, m.played < 0 ? 0 : m.played, lane);
