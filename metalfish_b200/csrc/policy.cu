@@ -325,13 +325,9 @@ struct Norm {
   float log_s, inv_s;
 };
 
-// Largest logit, and e[k] = exp(s - s_top) with this lane's part of `rest` and
-// of sum e s.
+// Sets top and live.
 template <int G>
-__device__ __forceinline__ Norm softmax_part(int n, const float (&z)[G], float inv_temp,
-                                             int lane, float (&e)[G],
-                                             float &es) {
-  Norm q;
+__device__ __forceinline__ void find_top(int n, const float (&z)[G], Norm &q) {
   float top = z[0];
 #pragma unroll
   for (int k = 1; k < G; ++k)
@@ -344,9 +340,27 @@ __device__ __forceinline__ Norm softmax_part(int n, const float (&z)[G], float i
     for (int k = 0; k < G; ++k) nan |= 32 * k < n && z[k] != z[k];
     q.live = __any_sync(kFull, nan);
   }
+}
+// Keeps one largest entry out of the sum, `mine` being this lane's lowest edge
+// with the largest logit, already kept out, or -1: every lane but the first that
+// has one puts it back. Sets lead.
+__device__ __forceinline__ void leave_one_out(int mine, int lane, Norm &q) {
+  const int first = __ffs(__ballot_sync(kFull, mine >= 0)) - 1;
+  if (mine >= 0 && lane != first) q.rest += 1.0f;
+  q.lead = lane == first ? mine : -1;
+}
+
+// Largest logit, and e[k] = exp(s - s_top) with this lane's part of `rest` and
+// of sum e s.
+template <int G>
+__device__ __forceinline__ Norm softmax_part(int n, const float (&z)[G], float inv_temp,
+                                             int lane, float (&e)[G],
+                                             float &es) {
+  Norm q;
+  find_top<G>(n, z, q);
   q.rest = 0.0f;
   es = 0.0f;
-  int mine = -1;  // this lane's lowest edge with the largest logit
+  int mine = -1;
 #pragma unroll
   for (int k = 0; k < G; ++k) {
     e[k] = 0.0f;
@@ -360,11 +374,7 @@ __device__ __forceinline__ Norm softmax_part(int n, const float (&z)[G], float i
         q.rest += e[k];
     }
   }
-  // every lane but the first that has one puts it back into the sum
-  const unsigned at = __ballot_sync(kFull, mine >= 0);
-  const int first = __ffs(at) - 1;
-  if (mine >= 0 && lane != first) q.rest += 1.0f;
-  q.lead = lane == first ? mine : -1;
+  leave_one_out(mine, lane, q);
   return q;
 }
 
@@ -573,17 +583,11 @@ __device__ __forceinline__ void write_nan_row(const Grad &out, int classes, int 
 }
 
 // ------------------------------------------------------------------ log-probabilities
-// kLines: the played move's log-probability goes into sums over long lines whose
-// differences are small, where what leans to one side adds up (the fast
-// exponential and the rounding of 1 / T do, by some 1e-8): it is made from the
-// accurate exponential, 1 / T in two parts and a 64-bit logarithm, and rounded
-// once. Its sign bit then tells whether the position takes part (set, for a NaN as
-// well) or has no move (+0), and row_grad gets the zero of a position in no line.
-template <int G, bool kLines, int kType>
+template <int G, int kType>
 __device__ __forceinline__ void score_position(const PolicyRows &r, int b,
                                                const Moves &m, int c0, int c1, int lane,
                                                float *move_logp, float *played_logp,
-                                               float *entropy, float *row_grad) {
+                                               float *entropy) {
   Edges<G> v;
   columns<G>(r, m, c0, c1, lane, v);
   unsigned bits[G];
@@ -606,40 +610,68 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, int b,
   }
   const bool takes = q.live && m.played >= 0;
   const float z = of_move<G>(v.z, m.played < 0 ? 0 : m.played, lane);
-  float logp = (z - q.top) * r.inv_temp - q.log_s;
-  if (kLines) {
-    float rest = 0.0f;
-#pragma unroll
-    for (int k = 0; k < G; ++k)
-      if (32 * k < m.n && 32 * k + lane != q.lead) {
-        const float d = v.z[k] - q.top;
-        if (!(d == -INFINITY)) rest += expf(fmaf(d, r.inv_temp, d * r.inv_temp_rest));
-      }
-    rest = warp_sum(rest);
-    if (q.top < INFINITY)  // (else it is NaN already)
-      logp = static_cast<float>((static_cast<double>(z) - q.top) / r.temp - log(1.0 + rest));
-  }
+  const float logp = (z - q.top) * r.inv_temp - q.log_s;
   if (lane == 0) {
-    const float value = m.bad ? quiet_nan() : takes ? logp : 0.0f;
-    // (a log-probability is never above 0)
-    if (kLines)
-      played_logp[b] = takes || m.bad ? __uint_as_float(__float_as_uint(value) | 0x80000000u) : 0.0f;
-    else if (played_logp)
-      played_logp[b] = value;
+    if (played_logp) played_logp[b] = m.bad ? quiet_nan() : takes ? logp : 0.0f;
     if (entropy) entropy[b] = m.bad ? quiet_nan() : q.live ? h : 0.0f;
-    if (kLines) row_grad[b] = 0.0f;
+  }
+}
+
+// The played move's log-probability for sums over long lines whose differences
+// are small, where what leans to one side adds up (the fast exponential and the
+// rounding of 1 / T do, by some 1e-8): it is made from the accurate exponential,
+// 1 / T in two parts and a 64-bit logarithm, and rounded once. Its sign bit tells
+// whether the position takes part (set, for a NaN as well) or has no move (+0).
+// row_grad gets the zero of a position in no line.
+template <int G, int kType>
+__device__ __forceinline__ void line_position(const PolicyRows &r, int b, const Moves &m, int c0,
+                                              int c1, int lane, float *played_logp,
+                                              float *row_grad) {
+  Edges<G> v;
+  columns<G>(r, m, c0, c1, lane, v);
+  unsigned bits[G];
+  const int type = type_of<kType>(r.type);
+  const void *row = row_of(r.logits, type, r.stride, b);
+  load_logits<G>(m.n, row, type, v.col, bits);
+  logits_of<G>(m.n, row, type, v.col, bits, v.z);
+  Norm q;
+  find_top<G>(m.n, v.z, q);
+  q.rest = 0.0f;
+  int mine = -1;
+#pragma unroll
+  for (int k = 0; k < G; ++k) {
+    if (32 * k < m.n) {
+      const float d = v.z[k] - q.top;
+      if (mine < 0 && v.z[k] == q.top)
+        mine = 32 * k + lane;
+      else if (!(d == -INFINITY))
+        q.rest += expf(fmaf(d, r.inv_temp, d * r.inv_temp_rest));
+    }
+  }
+  leave_one_out(mine, lane, q);
+  if (q.top == INFINITY) q.rest = quiet_nan();  // its own inf - inf is not in the sum
+  const double sum = 1.0 + warp_sum(q.rest);
+  const float z = of_move<G>(v.z, m.played < 0 ? 0 : m.played, lane);
+  const float logp = static_cast<float>((static_cast<double>(z) - q.top) * r.inv_temp64 - log(sum));
+  if (lane == 0) {
+    const float value = m.bad ? quiet_nan() : logp;
+    // (a log-probability is never above 0)
+    played_logp[b] = m.bad || (q.live && m.played >= 0)
+                         ? __uint_as_float(__float_as_uint(value) | 0x80000000u)
+                         : 0.0f;
+    row_grad[b] = 0.0f;
   }
 }
 
 // CTAs on an SM. 40 warps with 48 registers: 50021 bf16 positions take 21 us; with
 // 48 warps and 40 registers 22, with 32 warps and 64 registers 27. For lines, whose
-// 64-bit logarithm wants more registers, 4 and 5 are alike (96 pairs of games 44 and
-// 46 us, 256 pairs of short lines 20 and 19).
+// 64-bit logarithm wants more registers, 4 and 5 are alike (96 pairs of games 40 and
+// 41 us, 256 pairs of short lines 18.0 and 17.6).
 constexpr int kScoreCtas = 5, kLineCtas = 4;
-template <bool kLines, int kType>
-__global__ void __launch_bounds__(32 * kMaxWarps, kLines ? kLineCtas : kScoreCtas)
+template <int kType>
+__global__ void __launch_bounds__(32 * kMaxWarps, kScoreCtas)
     move_logprobs_kernel(const __grid_constant__ PolicyRows r, float *move_logp,
-                         float *played_logp, float *entropy, float *row_grad) {
+                         float *played_logp, float *entropy) {
   __shared__ Turns turns;
   start_turns(&turns);
   pdl_wait();
@@ -648,14 +680,32 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kLines ? kLineCtas : kScoreCta
   for_positions(
       r, gridDim.x, &turns,
       [&](int b, const Moves &m, int c0, int c1) {
-        score_position<2, kLines, kType>(r, b, m, c0, c1, lane, move_logp, played_logp, entropy,
-                                         row_grad);
+        score_position<2, kType>(r, b, m, c0, c1, lane, move_logp, played_logp, entropy);
         return false;
       },
       [&](int b, const Moves &m) {
-        score_position<8, kLines, kType>(r, b, m, load_index(r, m, 0, lane),
-                                         load_index(r, m, 1, lane), lane, move_logp, played_logp,
-                                         entropy, row_grad);
+        score_position<8, kType>(r, b, m, load_index(r, m, 0, lane), load_index(r, m, 1, lane),
+                                 lane, move_logp, played_logp, entropy);
+      });
+}
+
+template <int kType>
+__global__ void __launch_bounds__(32 * kMaxWarps, kLineCtas)
+    line_logprobs_kernel(const __grid_constant__ PolicyRows r, float *played_logp, float *row_grad) {
+  __shared__ Turns turns;
+  start_turns(&turns);
+  pdl_wait();
+  pdl_launch();
+  const int lane = threadIdx.x & 31;
+  for_positions(
+      r, gridDim.x, &turns,
+      [&](int b, const Moves &m, int c0, int c1) {
+        line_position<2, kType>(r, b, m, c0, c1, lane, played_logp, row_grad);
+        return false;
+      },
+      [&](int b, const Moves &m) {
+        line_position<8, kType>(r, b, m, load_index(r, m, 0, lane), load_index(r, m, 1, lane),
+                                lane, played_logp, row_grad);
       });
 }
 
@@ -972,20 +1022,34 @@ __global__ void __launch_bounds__(256)
     }
     return;
   }
+  const float w = scale * (weight ? weight[i] : 1.0f);
+  const unsigned first = at[0], cut = at[1], end = at[2];  // (unsigned: a step may pass 2^31)
   double sum[2] = {0.0, 0.0}, gain[2] = {0.0, 0.0};
+  for (unsigned from = first; from < end; from += 256) {  // sixteen loads under way at once
+    float lp[8], frozen[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const unsigned b = from + 32 * k + lane;
+      lp[k] = b < end ? logp[b] : 0.0f;
+      frozen[k] = b < end ? ref[b] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (from + 32 * k >= end) break;
+      const int side = from + 32 * k + lane < cut ? 0 : 1;
+      const double value = lp[k], up = signbit(lp[k]) ? value - frozen[k] : 0.0;
+      sum[0] += side ? 0.0 : value;
+      sum[1] += side ? value : 0.0;
+      gain[0] += side ? 0.0 : up;
+      gain[1] += side ? up : 0.0;
+    }
+  }
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
-#pragma unroll 4
-    for (int b = at[side] + lane; b < at[side + 1]; b += 32) {
-      const float lp = logp[b], frozen = ref[b];
-      sum[side] += static_cast<double>(lp);
-      gain[side] += signbit(lp) ? static_cast<double>(lp) - static_cast<double>(frozen) : 0.0;
-    }
     sum[side] = warp_sum(sum[side]);
     gain[side] = warp_sum(gain[side]);
   }
   const float mg = static_cast<float>(static_cast<double>(beta) * (gain[0] - gain[1]));
-  const float w = scale * (weight ? weight[i] : 1.0f);
   // -log sigma(m) = max(-m, 0) + log(1 + e^-|m|); sigma(-|m|) = e^-|m| / (1 + e^-|m|)
   const float tail = expf(-fabsf(mg));
   const float less = fmaxf(-mg, 0.0f) + log1pf(tail), more = fmaxf(mg, 0.0f) + log1pf(tail);
@@ -999,10 +1063,19 @@ __global__ void __launch_bounds__(256)
     // fmaxf drops a NaN margin: it is added back
     loss[i] = mg != mg ? mg : w * ((1.0f - eps) * less + eps * more);
   }
+  for (unsigned from = first; from < end; from += 256) {
+    float lp[8];
 #pragma unroll
-  for (int side = 0; side < 2; ++side)
-    for (int b = at[side] + lane; b < at[side + 1]; b += 32)
-      row_grad[b] = !signbit(logp[b]) ? 0.0f : side ? -slope : slope;
+    for (int k = 0; k < 8; ++k) {
+      const unsigned b = from + 32 * k + lane;
+      lp[k] = b < end ? logp[b] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const unsigned b = from + 32 * k + lane;
+      if (b < end) row_grad[b] = !signbit(lp[k]) ? 0.0f : b < cut ? slope : -slope;
+    }
+  }
 }
 
 // ------------------------------------------------------------------ total
@@ -1088,6 +1161,14 @@ cudaError_t launch_clip(const PolicyRows &r, const ClipArgs &a, cudaStream_t s) 
   return same ? with_type(r.type, launch) : launch(std::integral_constant<int, kAnyType>());
 }
 
+cudaError_t launch_lines(const PolicyRows &r, float *played_logp, float *row_grad, cudaStream_t s) {
+  const Shape t = shape_for(r.batch, kMaxWarps, kLineCtas, 0);
+  return with_type(r.type, [&](auto type) {
+    return launch_k(line_logprobs_kernel<decltype(type)::value>, dim3(t.ctas), dim3(32 * t.warps), 0,
+                    s, 1, r, played_logp, row_grad);
+  });
+}
+
 cudaError_t launch_pairs(int pairs, int batch, const int32_t *lines, const float *logp,
                          const float *ref, const float *weight, float beta, float eps, float scale,
                          float *row_grad, float *line_logp, float *margin, float *loss,
@@ -1108,13 +1189,11 @@ cudaError_t launch_total(const float *loss, int n, float *total, cudaStream_t s)
 }  // namespace
 
 cudaError_t launch_move_logprobs(const PolicyRows &r, float *move_logp, float *played_logp,
-                                 float *entropy, float *row_grad, cudaStream_t s) {
-  const Shape t = shape_for(r.batch, kMaxWarps, row_grad ? kLineCtas : kScoreCtas, 0);
+                                 float *entropy, cudaStream_t s) {
+  const Shape t = shape_for(r.batch, kMaxWarps, kScoreCtas, 0);
   return with_type(r.type, [&](auto type) {
-    constexpr int kType = decltype(type)::value;
-    return launch_k(row_grad ? move_logprobs_kernel<true, kType> : move_logprobs_kernel<false, kType>,
-                    dim3(t.ctas), dim3(32 * t.warps), 0, s, 1, r, move_logp, played_logp, entropy,
-                    row_grad);
+    return launch_k(move_logprobs_kernel<decltype(type)::value>, dim3(t.ctas), dim3(32 * t.warps), 0,
+                    s, 1, r, move_logp, played_logp, entropy);
   });
 }
 
@@ -1214,8 +1293,9 @@ PolicyRows rows_of(const mfb200_policy_rows &r) {
   o.num_moves = r.num_moves;
   o.played = r.played;
   o.temp = r.softmax_temp;
-  o.inv_temp = static_cast<float>(1.0 / r.softmax_temp);
-  o.inv_temp_rest = static_cast<float>(1.0 / r.softmax_temp - static_cast<double>(o.inv_temp));
+  o.inv_temp64 = 1.0 / r.softmax_temp;
+  o.inv_temp = static_cast<float>(o.inv_temp64);
+  o.inv_temp_rest = static_cast<float>(o.inv_temp64 - static_cast<double>(o.inv_temp));
   return o;
 }
 
@@ -1243,7 +1323,7 @@ extern "C" MFB200_API int mfb200_move_logprobs(const mfb200_policy_rows *rows, f
   if (!d_move_logp && !d_played_logp && !d_entropy) return fail(fn, "no output");
   if (const char *e = check_device(rows->logits)) return fail(fn, e);
   return launched(fn, launch_move_logprobs(rows_of(*rows), d_move_logp, d_played_logp, d_entropy,
-                                           nullptr, static_cast<cudaStream_t>(stream)));
+                                           static_cast<cudaStream_t>(stream)));
 }
 
 extern "C" MFB200_API int mfb200_move_logprobs_backward(
@@ -1382,7 +1462,7 @@ extern "C" MFB200_API int mfb200_preference_loss(
     if (const char *e = check_device(n > 0 ? rows->logits : d_line_offsets)) return fail(fn, e);
   const PolicyRows r = rows_of(*rows);
   cudaError_t e = cudaSuccess;
-  if (n > 0) e = launch_move_logprobs(r, nullptr, d_logp, nullptr, d_row_grad, s);
+  if (n > 0) e = launch_lines(r, d_logp, d_row_grad, s);
   if (e == cudaSuccess && pairs > 0)
     e = launch_pairs(pairs, n, d_line_offsets, d_logp, d_ref_logp, d_weight, cfg->beta,
                      cfg->label_smoothing, cfg->scale, d_row_grad, d_line_logp, d_margin, d_loss, s);

@@ -17,15 +17,13 @@ struct PolicyRows {
   const int16_t *index;   // [num_moves]
   long long num_moves;
   const int32_t *played;  // [batch] edge numbers, or null
-  double temp;
+  double temp, inv_temp64;
   float inv_temp, inv_temp_rest;  // 1 / temp in two parts
 };
 
 // Log-probabilities of the legal moves, of the played move and the entropy;
-// each output may be null. With row_grad the played moves' log-probabilities are
-// made for sums over long lines, their signs tell which positions take part, and
-// row_grad is set to zero (see score_position and preference_pair_kernel).
+// each output may be null.
 cudaError_t launch_move_logprobs(const PolicyRows &r, float *move_logp, float *played_logp,
-                                 float *entropy, float *row_grad, cudaStream_t s);
+                                 float *entropy, cudaStream_t s);
 
 }  // namespace mfb200

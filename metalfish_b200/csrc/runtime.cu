@@ -1482,10 +1482,9 @@ int eval_shard_logprobs(mfb200_handle *h, Shard &S, const uint64_t *masks, const
   r.index = S.move_idx;
   r.num_moves = nmoves;
   r.played = played ? S.played : nullptr;
-  r.temp = temp;
   r.inv_temp = static_cast<float>(1.0 / temp);
   check(launch_move_logprobs(r, move_logp ? S.priors : nullptr, played ? S.played_logp : nullptr,
-                             S.entropy, nullptr, s),
+                             S.entropy, s),
         "log-probabilities launch");
   check(cudaEventRecord(S.ev[2], s), "event");
   if (move_logp && nmoves > 0)
