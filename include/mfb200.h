@@ -424,7 +424,9 @@ typedef struct {
  *   loss[i] = scale * weight[i] * ( -(1 - eps) log sigma(margin) - eps log sigma(-margin) ).
  * A line may be empty (D = 0); positions in no line get a zero gradient. A
  * pair whose offsets decrease or leave the batch has NaN results. d_weight
- * NULL means 1. Written: d_logp [batch], d_row_grad [batch] (the gradient of
+ * NULL means 1. Written: d_logp [batch], d_logp_rest [batch] (what the rounding
+ * of d_logp leaves of the log-probability, which is made in 64 bits: the margin of
+ * lines that nearly cancel keeps its digits), d_row_grad [batch] (the gradient of
  * the total with respect to d_logp), d_line_logp [2 * pairs], d_margin, d_loss
  * [pairs]; optional d_total [1] and d_grad_logits as in
  * mfb200_move_logprobs_backward. */
@@ -432,8 +434,9 @@ MFB200_API int mfb200_preference_loss(const mfb200_policy_rows *rows,
                                       const mfb200_preference_config *cfg,
                                       const int32_t *d_line_offsets, int pairs,
                                       const float *d_ref_logp, const float *d_weight,
-                                      float *d_logp, float *d_row_grad, float *d_line_logp,
-                                      float *d_margin, float *d_loss, float *d_total,
+                                      float *d_logp, float *d_logp_rest, float *d_row_grad,
+                                      float *d_line_logp, float *d_margin, float *d_loss,
+                                      float *d_total,
                                       void *d_grad_logits, int64_t grad_stride, int grad_type,
                                       void *stream);
 MFB200_API const char *mfb200_policy_last_error(void);

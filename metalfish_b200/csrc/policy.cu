@@ -25,7 +25,7 @@
 // one bulk copy, while the warp goes on. 65536 positions, 1858 fp32 classes, on
 // B200: clipped loss with KL 128 us (615 MB of DRAM traffic; the same reads and
 // copies without any arithmetic 127 us, the copies alone 92), the backward pass
-// alone 111 us, log-probabilities 32 us.
+// alone 110 us, log-probabilities 28 us.
 #include "policy.cuh"
 
 #include <atomic>
@@ -617,16 +617,18 @@ __device__ __forceinline__ void score_position(const PolicyRows &r, int b,
   }
 }
 
-// The played move's log-probability for sums over long lines whose differences
-// are small, where what leans to one side adds up (the fast exponential and the
-// rounding of 1 / T do, by some 1e-8): it is made from the accurate exponential,
-// 1 / T in two parts and a 64-bit logarithm, and rounded once. Its sign bit tells
-// whether the position takes part (set, for a NaN as well) or has no move (+0).
-// row_grad gets the zero of a position in no line.
+// The played move's log-probability for sums over lines, whose difference is
+// small: made in 64 bits and given in two parts, the rounded value and the rest.
+// (From 32-bit exponentials the margin of a pair of 6-ply lines was 6e-7 of itself
+// off in the middle of 150 cases and 1e-5 in the worst.) The first part
+// tells whether the position takes part: +0 for one without a move, a set sign bit
+// or NaN for the others (takes_part). row_grad gets the zero of a position in no line.
+__device__ __forceinline__ bool takes_part(float logp) { return signbit(logp) || logp != logp; }
+
 template <int G, int kType>
 __device__ __forceinline__ void line_position(const PolicyRows &r, int b, const Moves &m, int c0,
                                               int c1, int lane, float *played_logp,
-                                              float *row_grad) {
+                                              float *logp_rest, float *row_grad) {
   Edges<G> v;
   columns<G>(r, m, c0, c1, lane, v);
   unsigned bits[G];
@@ -636,38 +638,26 @@ __device__ __forceinline__ void line_position(const PolicyRows &r, int b, const 
   logits_of<G>(m.n, row, type, v.col, bits, v.z);
   Norm q;
   find_top<G>(m.n, v.z, q);
-  q.rest = 0.0f;
-  int mine = -1;
+  double sum = 0.0;
 #pragma unroll
-  for (int k = 0; k < G; ++k) {
-    if (32 * k < m.n) {
-      const float d = v.z[k] - q.top;
-      if (mine < 0 && v.z[k] == q.top)
-        mine = 32 * k + lane;
-      else if (!(d == -INFINITY))
-        q.rest += expf(fmaf(d, r.inv_temp, d * r.inv_temp_rest));
-    }
-  }
-  leave_one_out(mine, lane, q);
-  if (q.top == INFINITY) q.rest = quiet_nan();  // its own inf - inf is not in the sum
-  const double sum = 1.0 + warp_sum(q.rest);
+  for (int k = 0; k < G; ++k)
+    if (32 * k < m.n) sum += exp((static_cast<double>(v.z[k]) - q.top) * r.inv_temp64);
+  sum = warp_sum(sum);
   const float z = of_move<G>(v.z, m.played < 0 ? 0 : m.played, lane);
-  const float logp = static_cast<float>((static_cast<double>(z) - q.top) * r.inv_temp64 - log(sum));
+  const double logp = (static_cast<double>(z) - q.top) * r.inv_temp64 - log(sum);
   if (lane == 0) {
-    const float value = m.bad ? quiet_nan() : logp;
-    // (a log-probability is never above 0)
-    played_logp[b] = m.bad || (q.live && m.played >= 0)
-                         ? __uint_as_float(__float_as_uint(value) | 0x80000000u)
-                         : 0.0f;
+    const bool takes = m.bad || (q.live && m.played >= 0);
+    const float value = m.bad ? quiet_nan() : static_cast<float>(logp);
+    played_logp[b] = takes ? copysignf(value, -1.0f) : 0.0f;  // never above 0
+    logp_rest[b] = takes && fabsf(value) < INFINITY ? static_cast<float>(logp - value) : 0.0f;
     row_grad[b] = 0.0f;
   }
 }
 
 // CTAs on an SM. 40 warps with 48 registers: 50021 bf16 positions take 21 us; with
-// 48 warps and 40 registers 22, with 32 warps and 64 registers 27. For lines, whose
-// 64-bit logarithm wants more registers, 4 and 5 are alike (96 pairs of games 40 and
-// 41 us, 256 pairs of short lines 18.0 and 17.6).
-constexpr int kScoreCtas = 5, kLineCtas = 4;
+// 48 warps and 40 registers 22, with 32 warps and 64 registers 27. The same for
+// lines: 96 pairs of games 42 us, 43 with 32 warps.
+constexpr int kScoreCtas = 5;
 template <int kType>
 __global__ void __launch_bounds__(32 * kMaxWarps, kScoreCtas)
     move_logprobs_kernel(const __grid_constant__ PolicyRows r, float *move_logp,
@@ -690,8 +680,9 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kScoreCtas)
 }
 
 template <int kType>
-__global__ void __launch_bounds__(32 * kMaxWarps, kLineCtas)
-    line_logprobs_kernel(const __grid_constant__ PolicyRows r, float *played_logp, float *row_grad) {
+__global__ void __launch_bounds__(32 * kMaxWarps, kScoreCtas)
+    line_logprobs_kernel(const __grid_constant__ PolicyRows r, float *played_logp, float *logp_rest,
+                         float *row_grad) {
   __shared__ Turns turns;
   start_turns(&turns);
   pdl_wait();
@@ -700,12 +691,12 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kLineCtas)
   for_positions(
       r, gridDim.x, &turns,
       [&](int b, const Moves &m, int c0, int c1) {
-        line_position<2, kType>(r, b, m, c0, c1, lane, played_logp, row_grad);
+        line_position<2, kType>(r, b, m, c0, c1, lane, played_logp, logp_rest, row_grad);
         return false;
       },
       [&](int b, const Moves &m) {
         line_position<8, kType>(r, b, m, load_index(r, m, 0, lane), load_index(r, m, 1, lane),
-                                lane, played_logp, row_grad);
+                                lane, played_logp, logp_rest, row_grad);
       });
 }
 
@@ -1000,12 +991,12 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3)
 // One warp per pair of lines. With D = the sum over a line's rows of
 // (logp - ref) and m = beta (D_preferred - D_rejected):
 //     L = scale w ( -(1 - eps) log sigma(m) - eps log sigma(-m) ),
-// and dL/dlogp of a row is +-beta dL/dm. A row whose logp has no sign bit takes no
-// part: its reference value is left out and its gradient zero. Rows in no line
+// and dL/dlogp of a row is +-beta dL/dm. A row that takes no part has its reference
+// value left out and a zero gradient. Rows in no line
 // keep the zero they have. The sums run in 64 bits, in an order fixed by the rows.
 __global__ void __launch_bounds__(256)
     preference_pair_kernel(int pairs, int batch, const int32_t *lines,
-                           const float *logp, const float *ref,
+                           const float *logp, const float *rest, const float *ref,
                            const float *weight, float beta, float eps, float scale,
                            float *row_grad, float *line_logp,
                            float *margin, float *loss) {
@@ -1025,19 +1016,21 @@ __global__ void __launch_bounds__(256)
   const float w = scale * (weight ? weight[i] : 1.0f);
   const unsigned first = at[0], cut = at[1], end = at[2];  // (unsigned: a step may pass 2^31)
   double sum[2] = {0.0, 0.0}, gain[2] = {0.0, 0.0};
-  for (unsigned from = first; from < end; from += 256) {  // sixteen loads under way at once
-    float lp[8], frozen[8];
+  for (unsigned from = first; from < end; from += 256) {  // 24 loads under way at once
+    float lp[8], low[8], frozen[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const unsigned b = from + 32 * k + lane;
       lp[k] = b < end ? logp[b] : 0.0f;
+      low[k] = b < end ? rest[b] : 0.0f;
       frozen[k] = b < end ? ref[b] : 0.0f;
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       if (from + 32 * k >= end) break;
       const int side = from + 32 * k + lane < cut ? 0 : 1;
-      const double value = lp[k], up = signbit(lp[k]) ? value - frozen[k] : 0.0;
+      const double value = static_cast<double>(lp[k]) + low[k];
+      const double up = takes_part(lp[k]) ? value - frozen[k] : 0.0;
       sum[0] += side ? 0.0 : value;
       sum[1] += side ? value : 0.0;
       gain[0] += side ? 0.0 : up;
@@ -1073,7 +1066,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const unsigned b = from + 32 * k + lane;
-      if (b < end) row_grad[b] = !signbit(lp[k]) ? 0.0f : b < cut ? slope : -slope;
+      if (b < end) row_grad[b] = !takes_part(lp[k]) ? 0.0f : b < cut ? slope : -slope;
     }
   }
 }
@@ -1161,22 +1154,23 @@ cudaError_t launch_clip(const PolicyRows &r, const ClipArgs &a, cudaStream_t s) 
   return same ? with_type(r.type, launch) : launch(std::integral_constant<int, kAnyType>());
 }
 
-cudaError_t launch_lines(const PolicyRows &r, float *played_logp, float *row_grad, cudaStream_t s) {
-  const Shape t = shape_for(r.batch, kMaxWarps, kLineCtas, 0);
+cudaError_t launch_lines(const PolicyRows &r, float *played_logp, float *logp_rest, float *row_grad,
+                         cudaStream_t s) {
+  const Shape t = shape_for(r.batch, kMaxWarps, kScoreCtas, 0);
   return with_type(r.type, [&](auto type) {
     return launch_k(line_logprobs_kernel<decltype(type)::value>, dim3(t.ctas), dim3(32 * t.warps), 0,
-                    s, 1, r, played_logp, row_grad);
+                    s, 1, r, played_logp, logp_rest, row_grad);
   });
 }
 
 cudaError_t launch_pairs(int pairs, int batch, const int32_t *lines, const float *logp,
-                         const float *ref, const float *weight, float beta, float eps, float scale,
+                         const float *rest, const float *ref, const float *weight, float beta, float eps, float scale,
                          float *row_grad, float *line_logp, float *margin, float *loss,
                          cudaStream_t s) {
   int w = 1;
   while (w < 8 && pairs > num_sms() * w) w *= 2;
   return launch_k(preference_pair_kernel, dim3((static_cast<unsigned>(pairs) + w - 1) / w),
-                  dim3(32 * w), 0, s, 1, pairs, batch, lines, logp, ref, weight, beta, eps, scale,
+                  dim3(32 * w), 0, s, 1, pairs, batch, lines, logp, rest, ref, weight, beta, eps, scale,
                   row_grad, line_logp, margin, loss);
 }
 
@@ -1295,7 +1289,6 @@ PolicyRows rows_of(const mfb200_policy_rows &r) {
   o.temp = r.softmax_temp;
   o.inv_temp64 = 1.0 / r.softmax_temp;
   o.inv_temp = static_cast<float>(o.inv_temp64);
-  o.inv_temp_rest = static_cast<float>(o.inv_temp64 - static_cast<double>(o.inv_temp));
   return o;
 }
 
@@ -1419,8 +1412,9 @@ extern "C" MFB200_API int mfb200_clipped_policy_loss(
 extern "C" MFB200_API int mfb200_preference_loss(
     const mfb200_policy_rows *rows, const mfb200_preference_config *cfg,
     const int32_t *d_line_offsets, int pairs, const float *d_ref_logp, const float *d_weight,
-    float *d_logp, float *d_row_grad, float *d_line_logp, float *d_margin, float *d_loss,
-    float *d_total, void *d_grad_logits, int64_t grad_stride, int grad_type, void *stream) {
+    float *d_logp, float *d_logp_rest, float *d_row_grad, float *d_line_logp, float *d_margin,
+    float *d_loss, float *d_total, void *d_grad_logits, int64_t grad_stride, int grad_type,
+    void *stream) {
   const char *fn = "mfb200_preference_loss";
   if (!rows || !cfg) return fail(fn, "null rows or config");
   if (rows->batch < 0 || pairs < 0) return fail(fn, "negative batch or number of pairs");
@@ -1434,10 +1428,10 @@ extern "C" MFB200_API int mfb200_preference_loss(
     return fail(fn, "label_smoothing must be between 0 and 1");
   if (pairs > 0 && (!d_line_offsets || !d_line_logp || !d_margin || !d_loss))
     return fail(fn, "null line_offsets, line_logp, margin or loss");
-  if (rows->batch > 0 && (!d_ref_logp || !d_logp || !d_row_grad))
-    return fail(fn, "null ref_logp, logp or row_grad");
+  if (rows->batch > 0 && (!d_ref_logp || !d_logp || !d_logp_rest || !d_row_grad))
+    return fail(fn, "null ref_logp, logp, logp_rest or row_grad");
   const int n = rows->batch;
-  const void *per_row[] = {d_ref_logp, d_logp, d_row_grad};
+  const void *per_row[] = {d_ref_logp, d_logp, d_logp_rest, d_row_grad};
   const void *per_pair[] = {d_weight, d_margin, d_loss};
   for (const void *p : per_row)
     if (!aligned(p, 4)) return fail(fn, "an array is not aligned to its element type");
@@ -1462,9 +1456,9 @@ extern "C" MFB200_API int mfb200_preference_loss(
     if (const char *e = check_device(n > 0 ? rows->logits : d_line_offsets)) return fail(fn, e);
   const PolicyRows r = rows_of(*rows);
   cudaError_t e = cudaSuccess;
-  if (n > 0) e = launch_lines(r, d_logp, d_row_grad, s);
+  if (n > 0) e = launch_lines(r, d_logp, d_logp_rest, d_row_grad, s);
   if (e == cudaSuccess && pairs > 0)
-    e = launch_pairs(pairs, n, d_line_offsets, d_logp, d_ref_logp, d_weight, cfg->beta,
+    e = launch_pairs(pairs, n, d_line_offsets, d_logp, d_logp_rest, d_ref_logp, d_weight, cfg->beta,
                      cfg->label_smoothing, cfg->scale, d_row_grad, d_line_logp, d_margin, d_loss, s);
   const bool with_grad = n > 0 && d_grad_logits;
   if (e == cudaSuccess && with_grad) {

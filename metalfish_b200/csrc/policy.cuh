@@ -17,8 +17,8 @@ struct PolicyRows {
   const int16_t *index;   // [num_moves]
   long long num_moves;
   const int32_t *played;  // [batch] edge numbers, or null
-  double temp, inv_temp64;
-  float inv_temp, inv_temp_rest;  // 1 / temp in two parts
+  double temp, inv_temp64;  // 1 / temp
+  float inv_temp;
 };
 
 // Log-probabilities of the legal moves, of the played move and the entropy;

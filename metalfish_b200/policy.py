@@ -98,7 +98,7 @@ def _lib():
         L.mfb200_preference_loss.restype = _int
         L.mfb200_preference_loss.argtypes = [
             rows, ctypes.POINTER(_PreferenceConfig), _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
-            _vp, _vp, _i64, _int, _vp]
+            _vp, _vp, _vp, _i64, _int, _vp]
         _native = L
     return _native
 
@@ -271,10 +271,12 @@ def preference_loss(logits, move_offsets, move_index, played, line_offsets, ref_
     g, ptr, stride, kind = _gradient(logits, shape, grad, grad_logits, device)
     cfg = _PreferenceConfig(beta, label_smoothing, scale if scale is not None else 1.0 / max(pairs, 1))
     total = ref_logp.new_empty(())
-    logp, row_grad = torch.empty_like(ref_logp), torch.empty_like(ref_logp)
-    loss, margin = ref_logp.new_empty(pairs), ref_logp.new_empty(pairs)
+    logp, rest, row_grad = (torch.empty_like(ref_logp), torch.empty_like(ref_logp),
+                            torch.empty_like(ref_logp))
+    loss = ref_logp.new_empty(pairs)
+    margin = torch.empty_like(loss)
     line_logp = ref_logp.new_empty(2 * pairs)
     _call(L.mfb200_preference_loss, device, rows, cfg, lines, pairs, ref, w, logp.data_ptr(),
-          row_grad.data_ptr(), line_logp.data_ptr(), margin.data_ptr(), loss.data_ptr(),
+          rest.data_ptr(), row_grad.data_ptr(), line_logp.data_ptr(), margin.data_ptr(), loss.data_ptr(),
           total.data_ptr(), ptr, stride, kind)
     return PreferenceLoss(total, loss, margin, line_logp, logp, row_grad, g)

@@ -38,10 +38,11 @@ def clip(r, cfg=(0.2, 0.2, 0.0, 0.0, 1.0), old=5 * A, adv=6 * A, w=None, ref=Non
 
 
 def prefer(r, cfg=(0.1, 0.0, 1.0), lines=5 * A, pairs=2, ref=6 * A, w=None, logp=7 * A, row_grad=8 * A,
-           line_logp=9 * A, margin=10 * A, loss=11 * A, total=12 * A, grad=G, stride=1858, kind=0):
+           line_logp=9 * A, margin=10 * A, loss=11 * A, total=12 * A, rest=13 * A, grad=G, stride=1858,
+           kind=0):
     return policy._lib().mfb200_preference_loss(
-        r, policy._PreferenceConfig(*cfg), lines, pairs, ref, w, logp, row_grad, line_logp, margin,
-        loss, total, grad, stride, kind, None)
+        r, policy._PreferenceConfig(*cfg), lines, pairs, ref, w, logp, rest, row_grad, line_logp,
+        margin, loss, total, grad, stride, kind, None)
 
 
 ROWS = [(dict(classes=0), "classes"), (dict(classes=32768, logits_stride=40000), "classes"),
@@ -70,7 +71,7 @@ def test_null_structs():
     refused(L.mfb200_move_logprobs(None, A, A, A, None), "null rows")
     refused(L.mfb200_move_logprobs_backward(None, A, A, A, G, 1858, 0, None), "null rows")
     refused(L.mfb200_clipped_policy_loss(None, None, *[None] * 4, 0, 0, *[None] * 6, 0, 0, None), "null rows")
-    refused(L.mfb200_preference_loss(None, None, None, 0, *[None] * 9, 0, 0, None), "null rows")
+    refused(L.mfb200_preference_loss(None, None, None, 0, *[None] * 10, 0, 0, None), "null rows")
 
 
 def test_move_logprobs_refusals():
@@ -128,7 +129,7 @@ def test_preference_refusals():
     refused(prefer(rows(played=None)), "played")
     refused(prefer(rows(), pairs=-1), "negative")
     refused(prefer(rows(), pairs=1 << 30), "too many")
-    for name in ("lines", "line_logp", "margin", "loss", "ref", "logp", "row_grad"):
+    for name in ("lines", "line_logp", "margin", "loss", "ref", "logp", "rest", "row_grad"):
         refused(prefer(rows(), **{name: None}), "null")
         refused(prefer(rows(), **{name: A + 2}), "aligned")
         refused(prefer(rows(), **{name: G}), "overlaps")

@@ -326,6 +326,22 @@ def test_preference_margins_of_long_lines():
     check_preference(x, out, rows, logp, frozen, [0, 800, 1200], 0.1, 0.0, [1.0], 1.0)
 
 
+@pytest.mark.parametrize("temp", [1.0, 1.93])
+def test_preference_margins_of_lines_that_cancel(temp):
+    """References that are the rounded log-probabilities themselves leave some
+    1e-7 of each line. A row's log-probability is made in 64 bits (exponentials,
+    logarithm, arguments below 20 and eight additions: 50 steps of 2^-52, and as
+    many in the oracle) and its rest is rounded once, U |rest| <= U^2 |logp|."""
+    x = Batch("f32", 1858, [31, 2, 64, 218, 1, 33, 20, 40, 7, 0, 65, 30], 31, temp)
+    rows, logp, _, lines = line_case(x, [0, 6, 12])
+    frozen = logp.astype(np.float32)
+    out = policy.preference_loss(*x.args(), lines, x.f32(frozen), beta=1.0, softmax_temp=temp)
+    gain = logp - frozen.astype(np.float64)
+    margin = gain[:6].sum() - gain[6:].sum()
+    off = np.sum(ref.U ** 2 * np.abs(logp) + 100 * 2.0 ** -52)
+    assert abs(out.margin.item() - margin) <= off + ref.U * abs(margin)
+
+
 @pytest.mark.parametrize("pairs,plies", [(1, 1), (300, 4), (2, 700), (1300, 1)])
 def test_preference_loss_sizes(pairs, plies):
     rng = np.random.default_rng(pairs)
@@ -684,7 +700,7 @@ def test_the_calls_allocate_nothing():
             p[0], p[1], None, p[2], total.data_ptr(), grad.data_ptr(), 1858, 0, None) == 0
         assert L.mfb200_preference_loss(
             rows, policy._PreferenceConfig(0.1, 0.0, 1.0), lines.data_ptr(), 25, z.data_ptr(), None, p[0], p[1],
-            p[2], p[3], p[4], total.data_ptr(), grad.data_ptr(), 1858, 0, None) == 0
+            p[2], p[3], p[4], p[5], total.data_ptr(), grad.data_ptr(), 1858, 0, None) == 0
 
     calls()
     torch.cuda.synchronize()
