@@ -422,6 +422,10 @@ typedef struct {
  * a line's positions that have a played move:
  *   margin[i] = beta * (D_preferred - D_rejected),
  *   loss[i] = scale * weight[i] * ( -(1 - eps) log sigma(margin) - eps log sigma(-margin) ).
+ * A term whose coefficient (beta, 1 - eps, eps) is 0 is left out. A log-probability
+ * or reference value of -inf makes the margin infinite: its loss is then 0 or
+ * infinite, as the terms that are left are, and its gradient finite (NaN where both
+ * lines' D are infinite alike).
  * A line may be empty (D = 0); positions in no line get a zero gradient. A
  * pair whose offsets decrease or leave the batch has NaN results. d_weight
  * NULL means 1. Written: d_logp [batch], d_logp_rest [batch] (what the rounding

@@ -1042,7 +1042,8 @@ __global__ void __launch_bounds__(256)
     sum[side] = warp_sum(sum[side]);
     gain[side] = warp_sum(gain[side]);
   }
-  const float mg = static_cast<float>(static_cast<double>(beta) * (gain[0] - gain[1]));
+  // A term whose coefficient is 0 is left out, so that it is 0 where the margin is infinite.
+  const float mg = beta == 0.0f ? 0.0f : static_cast<float>(static_cast<double>(beta) * (gain[0] - gain[1]));
   // -log sigma(m) = max(-m, 0) + log(1 + e^-|m|); sigma(-|m|) = e^-|m| / (1 + e^-|m|)
   const float tail = expf(-fabsf(mg));
   const float less = fmaxf(-mg, 0.0f) + log1pf(tail), more = fmaxf(mg, 0.0f) + log1pf(tail);
@@ -1054,7 +1055,7 @@ __global__ void __launch_bounds__(256)
     line_logp[2 * i + 1] = static_cast<float>(sum[1]);
     margin[i] = mg;
     // fmaxf drops a NaN margin: it is added back
-    loss[i] = mg != mg ? mg : w * ((1.0f - eps) * less + eps * more);
+    loss[i] = mg != mg ? mg : w * ((eps < 1.0f ? (1.0f - eps) * less : 0.0f) + (eps > 0.0f ? eps * more : 0.0f));
   }
   for (unsigned from = first; from < end; from += 256) {
     float lp[8];

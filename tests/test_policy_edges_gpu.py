@@ -1,0 +1,66 @@
+"""Infinities, switched-off terms, far offsets and rows that take no part, in
+the policy operators: against their formulas in 64 bits."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from metalfish_b200 import policy  # noqa: E402
+from tests import policy_reference as ref  # noqa: E402
+from tests.test_policy_ops_gpu import Batch, check_clip, clip_case, line_case, near  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+INF = np.inf
+
+
+def play(x, at):
+    x.played_host[:] = at
+    x.played.copy_(torch.from_numpy(x.played_host))
+
+
+def terms(m, eps):
+    """-(1 - eps) log sigma(m) - eps log sigma(-m), without the term whose
+    coefficient is 0: the definition at an infinite margin."""
+    return ((1 - eps) * np.logaddexp(0, -m) if eps < 1 else 0.0) + (eps * np.logaddexp(0, m) if eps > 0 else 0.0)
+
+
+@pytest.mark.parametrize("eps", [0.0, 0.25, 1.0])
+def test_preference_with_infinite_margins(eps):
+    """A played move of logit -inf (log-probability -inf) in the rejected or
+    the preferred line, and a reference value of -inf in either: the margin is
+    infinite, the loss is 0 where only the term that is left has a coefficient."""
+    x = Batch("f32", 1858, [20] * 12, 40)
+    play(x, 3)
+    for b in (3, 4):  # rejected move of pair 1, preferred one of pair 2
+        x.logits[b, int(x.lists[b][3])] = -INF
+    rows, logp, frozen, lines = line_case(x, np.arange(13))
+    frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
+    frozen[6] = frozen[9] = -INF  # preferred of pair 3, rejected of pair 4
+    want = [None, INF, -INF, INF, -INF, None]
+    scale = 3.0
+    out = policy.preference_loss(*x.args(), lines, x.f32(frozen), beta=0.4, label_smoothing=eps, scale=scale)
+    for i, m in enumerate(want):
+        got, loss = out.margin[i].item(), out.loss[i].item()
+        if m is None:
+            assert np.isfinite(got) and np.isfinite(loss)
+            continue
+        assert got == m
+        assert loss == scale * terms(m, eps), (i, loss)
+        # sigma(m) and sigma(-m) are 0 and 1: U covers the one product's rounding
+        slope = scale * 0.4 * (eps * (m > 0) - (1 - eps) * (m < 0))
+        near(out.row_grad[2 * i:2 * i + 2].cpu().numpy(), [slope, -slope], 4 * ref.U * abs(slope), "row_grad")
+    assert torch.isfinite(out.grad_logits).all()
+    finite = torch.isfinite(out.loss)
+    total = out.loss.double().sum().item()
+    assert (out.total.item() == INF) if not finite.all() else abs(out.total.item() - total) <= 2 * ref.U * abs(total)
+
+
+def test_preference_without_a_margin():
+    """beta 0 takes the margin out, an infinite one too."""
+    x = Batch("f32", 1858, [20] * 2, 41)
+    play(x, 3)
+    x.logits[1, int(x.lists[1][3])] = -INF
+    lines = torch.arange(3, dtype=torch.int32, device="cuda")
+    out = policy.preference_loss(*x.args(), lines, torch.zeros(2, device="cuda"), beta=0.0)
+    assert out.margin.item() == 0 and (out.grad_logits == 0).all()
+    near(out.loss.item(), np.log(2), 4 * ref.U)
