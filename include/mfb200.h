@@ -398,7 +398,8 @@ typedef struct {
  * d_grad_logits as in mfb200_move_logprobs_backward. A reference logit of -inf
  * at a move that the policy gives a probability makes the KL infinite (and the
  * gradient of the row infinite or NaN, as the formula is); a reference without
- * any move above -inf, or with NaN or +inf among them, makes it NaN. */
+ * any move above -inf, or with NaN or +inf among them, makes it NaN. With
+ * kl_coef 0 the KL is given but takes no part, whatever it is. */
 MFB200_API int mfb200_clipped_policy_loss(const mfb200_policy_rows *rows,
                                           const mfb200_clip_config *cfg, const float *d_old_logp,
                                           const float *d_advantage, const float *d_weight,

@@ -879,6 +879,7 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   if (a.ref) load_logits<G>(m.n, ref, ref_type, v.col, ref_bits);
   const float old = a.old_logp[b], adv = a.advantage[b];
   const float c = a.scale * (a.weight ? a.weight[b] : 1.0f);
+  const bool kl_counts = a.ref && a.kl_coef != 0.0f;  // 0 times an infinite KL is no term
   logits_of<G>(m.n, row, type, v.col, bits, v.z);
   if (a.ref) logits_of<G>(m.n, ref, ref_type, v.col, ref_bits, d);
   float es;
@@ -929,7 +930,7 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
       const float p = v.e[k] * q.inv_s;
       float t = slope * played_term(m, q, 32 * k + lane, p);
       if (p != 0.0f) {
-        if (a.ref) t += a.kl_coef * p * (d[k] - kl);
+        if (kl_counts) t += a.kl_coef * p * (d[k] - kl);
         t += a.entropy_coef * p * ((v.z[k] - q.top) * r.inv_temp - q.log_s + h);
       }
       g[k] = c * r.inv_temp * t;
@@ -940,7 +941,7 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   // after the row: the fence before its copy would wait for these stores
   if (lane == 0) {
     float loss = -adv * (active ? ratio : border);
-    if (a.ref) loss += a.kl_coef * kl;
+    if (kl_counts) loss += a.kl_coef * kl;
     loss -= a.entropy_coef * h;
     if (a.loss) a.loss[b] = takes ? c * loss : 0.0f;
     if (a.logp) a.logp[b] = takes ? sa - q.log_s : 0.0f;

@@ -35,6 +35,7 @@ def test_preference_with_infinite_margins(eps):
         x.logits[b, int(x.lists[b][3])] = -INF
     rows, logp, frozen, lines = line_case(x, np.arange(13))
     frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
+    frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
     frozen[6] = frozen[9] = -INF  # preferred of pair 3, rejected of pair 4
     want = [None, INF, -INF, INF, -INF, None]
     scale = 3.0
@@ -64,3 +65,20 @@ def test_preference_without_a_margin():
     out = policy.preference_loss(*x.args(), lines, torch.zeros(2, device="cuda"), beta=0.0)
     assert out.margin.item() == 0 and (out.grad_logits == 0).all()
     near(out.loss.item(), np.log(2), 4 * ref.U)
+
+
+@pytest.mark.parametrize("value", [-INF, INF, np.nan])
+@pytest.mark.parametrize("dtype,ref_dtype", [("f32", "f32"), ("bf16", "f32")])
+def test_kl_is_watched_without_taking_part(value, dtype, ref_dtype):
+    """With kl_coef 0 the KL is given and is no part of the loss, whatever it is."""
+    x = Batch(dtype, 1858, [40, 70, 0, 20], 42)
+    play(x, [3, 66, -1, 5])
+    rows, other, old, adv, w = clip_case(x, True, ref_dtype)
+    for b in (0, 1, 3):
+        other[b, int(x.lists[b][9])] = value
+    args = x.f32(old), x.f32(adv)
+    out = policy.clipped_policy_loss(*x.args(), *args, ref_logits=other, weight=x.f32(w), entropy_coef=0.02)
+    kl = out.kl.cpu().numpy()
+    assert kl[2] == 0
+    assert np.all(kl[[0, 1, 3]] == INF) if value == -INF else np.isnan(kl[[0, 1, 3]]).all()
+    check_clip(x, out, rows, None, old, adv, w, 0.2, 0.2, 0.0, 0.02, 0.25)
