@@ -391,7 +391,8 @@ typedef struct {
  * KL = sum p (log p - log q) over the legal moves against the softmax q of
  * d_ref_logits ([batch, classes], rows ref_stride apart, ref_type; same
  * softmax_temp; NULL for no KL term), H the entropy. d_weight NULL means 1. A
- * position without a played move has loss 0 and a zero gradient. The clip is
+ * position without a played move has loss 0 and a zero gradient. An advantage of 0
+ * makes the first term 0, also where the ratio overflows. The clip is
  * decided in 64 bits; at its border the gradient is the unclipped one.
  * Outputs, each may be NULL: d_loss, d_logp (0 without a played move), d_kl,
  * d_entropy [batch]; d_total [1], the sum of d_loss (needs d_loss);

@@ -904,7 +904,8 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   const bool takes = q.live && m.played >= 0;
   const float za = of_move<G>(v.z, m.played < 0 ? 0 : m.played, lane);
   const float sa = (za - q.top) * r.inv_temp;
-  const float ratio = exp_fast((sa - old) - q.log_s);
+  float ratio = exp_fast((sa - old) - q.log_s);
+  if (adv == 0.0f && ratio == INFINITY) ratio = 1.0f;  // the surrogate is 0 for any ratio
   // The gradient jumps where the ratio crosses the clip's border, so a ratio
   // within the rounding of the border is computed again in 64 bits.
   const float border = static_cast<float>(adv > 0.0f ? a.high : a.low);

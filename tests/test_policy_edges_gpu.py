@@ -36,6 +36,7 @@ def test_preference_with_infinite_margins(eps):
     rows, logp, frozen, lines = line_case(x, np.arange(13))
     frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
     frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
+    frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
     frozen[6] = frozen[9] = -INF  # preferred of pair 3, rejected of pair 4
     want = [None, INF, -INF, INF, -INF, None]
     scale = 3.0
@@ -82,3 +83,22 @@ def test_kl_is_watched_without_taking_part(value, dtype, ref_dtype):
     assert kl[2] == 0
     assert np.all(kl[[0, 1, 3]] == INF) if value == -INF else np.isnan(kl[[0, 1, 3]]).all()
     check_clip(x, out, rows, None, old, adv, w, 0.2, 0.2, 0.0, 0.02, 0.25)
+
+
+def test_advantage_of_zero_with_a_ratio_out_of_range():
+    """-min(r A, clip(r) A) is 0 for A = 0, also where r overflows 32 bits or is infinite."""
+    x = Batch("f32", 1858, [20] * 4, 43)
+    play(x, 3)
+    old = np.array([-200.0, -INF, -90.0, -3.0], np.float32)
+    zero = torch.zeros(4, device="cuda")
+    out = policy.clipped_policy_loss(*x.args(), x.f32(old), zero, entropy_coef=0.5, scale=1.0)
+    rows = x.rows()
+    for b, row in enumerate(rows):
+        near(out.loss[b].item(), -0.5 * row.h, row.slack * ref.U * (1 + 2 * row.h), f"loss {b}")
+    g = np.zeros((4, 1858))
+    off = np.zeros((4, 1858))
+    for b, row in enumerate(rows):
+        v, m = row.backward(np.zeros(20), 0.0, 3, -0.5)
+        g[b] = row.dense(v, 1858)
+        off[b] = row.dense(row.slack * ref.U * m, 1858)
+    near(out.grad_logits.cpu().numpy(), g, off + ref.U * np.abs(g), "grad")
