@@ -892,8 +892,11 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
 #pragma unroll
     for (int k = 0; k < G; ++k) {
       if (32 * k < m.n) {
-        // the near logits are subtracted first
-        d[k] = ((v.z[k] - d[k]) - (q.top - w.top)) * r.inv_temp + (w.log_s - q.log_s);
+        // Both rows' gaps to their largest logit are nearly exact in 64 bits, and so is
+        // their difference: of near policies, and of logits with a number of their own
+        // added to each row (in 32 bits the two needs exclude each other).
+        const double gap = (static_cast<double>(v.z[k]) - q.top) - (static_cast<double>(d[k]) - w.top);
+        d[k] = static_cast<float>(gap) * r.inv_temp + (w.log_s - q.log_s);
         kl += kl_term(v.e[k] * q.inv_s, er[k] * w.inv_s, d[k]);
       }
     }

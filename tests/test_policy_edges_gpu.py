@@ -37,6 +37,7 @@ def test_preference_with_infinite_margins(eps):
     frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
     frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
     frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
+    frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
     frozen[6] = frozen[9] = -INF  # preferred of pair 3, rejected of pair 4
     want = [None, INF, -INF, INF, -INF, None]
     scale = 3.0
@@ -102,3 +103,41 @@ def test_advantage_of_zero_with_a_ratio_out_of_range():
         g[b] = row.dense(v, 1858)
         off[b] = row.dense(row.slack * ref.U * m, 1858)
     near(out.grad_logits.cpu().numpy(), g, off + ref.U * np.abs(g), "grad")
+
+
+@pytest.mark.parametrize("shift", [65536.0, -1e6, 3e7])
+@pytest.mark.parametrize("which", ["policy", "reference"])
+def test_kl_of_logits_with_an_offset_of_their_own(shift, which):
+    """A softmax does not see a number that is added to a whole row. The given
+    32-bit logits are the oracle's too, so its bounds hold unchanged: each
+    logit minus its row's largest is exact or off by U of itself."""
+    x = Batch("f32", 1858, [40, 64, 90, 2] * 8, 44)
+    rows, other, old, adv, w = clip_case(x)
+    if which == "policy":
+        x.logits = x.logits + shift
+    else:
+        other = other + shift
+    rows = x.rows()
+    old = np.array([r.logp[a] if a >= 0 else 0.0 for r, a in zip(rows, x.played_host)], np.float32) - np.float32(0.1)
+    out = policy.clipped_policy_loss(*x.args(), x.f32(old), x.f32(adv), ref_logits=other, weight=x.f32(w), kl_coef=0.3,
+                                     entropy_coef=0.01)
+    check_clip(x, out, rows, x.rows(other), old, adv, w, 0.2, 0.2, 0.3, 0.01, 1.0 / x.n)
+
+
+@pytest.mark.parametrize("which", ["policy", "reference", "both"])
+def test_kl_where_every_listed_logit_is_the_lowest(which):
+    """A mask of the type's lowest value over a whole list makes it uniform."""
+    x = Batch("f32", 1858, [40] * 4, 45)
+    play(x, 3)
+    rows, other, old, adv, w = clip_case(x)
+    low = torch.finfo(torch.float32).min
+    for b in (1, 2):
+        at = torch.from_numpy(np.asarray(x.lists[b], np.int64)).cuda()
+        if which != "reference":
+            x.logits[b, at] = low
+        if which != "policy":
+            other[b, at] = low
+    rows = x.rows()
+    old = np.array([r.logp[3] for r in rows], np.float32)
+    out = policy.clipped_policy_loss(*x.args(), x.f32(old), x.f32(adv), ref_logits=other, weight=x.f32(w), kl_coef=0.3)
+    check_clip(x, out, rows, x.rows(other), old, adv, w, 0.2, 0.2, 0.3, 0.0, 0.25)
