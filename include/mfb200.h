@@ -391,7 +391,8 @@ typedef struct {
  * KL = sum p (log p - log q) over the legal moves against the softmax q of
  * d_ref_logits ([batch, classes], rows ref_stride apart, ref_type; same
  * softmax_temp; NULL for no KL term), H the entropy. d_weight NULL means 1. A
- * position without a played move has loss 0 and a zero gradient. An advantage of 0
+ * position without a played move has loss 0 and a zero gradient, whatever its
+ * logits hold. An advantage of 0
  * makes the first term 0, also where the ratio overflows. The clip is
  * decided in 64 bits; at its border the gradient is the unclipped one.
  * Outputs, each may be NULL: d_loss, d_logp (0 without a played move), d_kl,
@@ -428,7 +429,9 @@ typedef struct {
  * or reference value of -inf makes the margin infinite: its loss is then 0 or
  * infinite, as the terms that are left are, and its gradient finite (NaN where both
  * lines' D are infinite alike).
- * A line may be empty (D = 0); positions in no line get a zero gradient. A
+ * A line may be empty (D = 0). Positions in no line, and those without a played
+ * move, get a zero gradient, also where their logits hold NaN or +inf (a malformed
+ * position gets NaN all the same). A
  * pair whose offsets decrease or leave the batch has NaN results. d_weight
  * NULL means 1. Written: d_logp [batch], d_logp_rest [batch] (what the rounding
  * of d_logp leaves of the log-probability, which is made in 64 bits: the margin of

@@ -710,6 +710,7 @@ __device__ __forceinline__ float played_term(const Moves &m, const Norm &q, int 
 // move's and g_H of the entropy, each of which may be null.
 struct BackArgs {
   const float *moves, *played, *entropy;
+  bool parts_only;  // a row whose upstream gradient is 0 takes no part: a zero row, whatever its logits are
   Grad out;
   // the sum of n losses, by one more CTA, where `total` is set
   const float *loss;
@@ -739,6 +740,7 @@ __device__ __forceinline__ void back_position(const PolicyRows &r, const BackArg
   float es;
   Norm q = softmax_part<G>(m.n, v.z, r.inv_temp, lane, v.e, es);
   const float h = softmax_done<Sums::kMore>(q, es, q, total, lane);
+  const bool takes = q.live && !(a.parts_only && ga == 0.0f);
 #pragma unroll
   for (int k = 0; k < G; ++k) {
     if (32 * k >= m.n) continue;
@@ -747,7 +749,7 @@ __device__ __forceinline__ void back_position(const PolicyRows &r, const BackArg
     float t = g[k] - p * total + ga * played_term(m, q, j, p);
     if (a.entropy && p != 0.0f) t -= gh * p * ((v.z[k] - q.top) * r.inv_temp - q.log_s + h);
     g[k] = t * r.inv_temp;
-    if (!q.live) v.col[k] = kNoColumn;
+    if (!takes) v.col[k] = kNoColumn;
   }
   write_row<G, kType>(im, a.out, r.classes, b, m.n, lane, v.col, g);
 }
@@ -1470,6 +1472,7 @@ extern "C" MFB200_API int mfb200_preference_loss(
   if (e == cudaSuccess && with_grad) {
     BackArgs a{};
     a.played = d_row_grad;
+    a.parts_only = true;
     a.out = Grad{d_grad_logits, grad_stride, grad_type};
     if (pairs > 0 && d_total) {
       a.loss = d_loss;

@@ -38,6 +38,7 @@ def test_preference_with_infinite_margins(eps):
     frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
     frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
     frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
+    frozen[[3, 4]] = -3.0  # (from line_case they are -inf too, and the difference undefined)
     frozen[6] = frozen[9] = -INF  # preferred of pair 3, rejected of pair 4
     want = [None, INF, -INF, INF, -INF, None]
     scale = 3.0
@@ -141,3 +142,26 @@ def test_kl_where_every_listed_logit_is_the_lowest(which):
     old = np.array([r.logp[3] for r in rows], np.float32)
     out = policy.clipped_policy_loss(*x.args(), x.f32(old), x.f32(adv), ref_logits=other, weight=x.f32(w), kl_coef=0.3)
     check_clip(x, out, rows, x.rows(other), old, adv, w, 0.2, 0.2, 0.3, 0.0, 0.25)
+
+
+@pytest.mark.parametrize("value", [np.nan, INF])
+def test_positions_that_take_no_part_have_no_gradient(value):
+    """Padding of any content, in a line without a played move or in no line:
+    its gradient is 0 and the pairs do not see it."""
+    x = Batch("f32", 1858, [20, 70, 20, 20, 20, 90, 20], 46)
+    play(x, [3, -1, -1, 2, 5, 6, 7])
+    lines = torch.tensor([0, 3, 5], dtype=torch.int32, device="cuda")  # 5 and 6 are in no line
+    frozen = torch.full((7,), -3.0, device="cuda")
+    want = policy.preference_loss(*x.args(), lines, frozen)
+    for b in (1, 2, 5, 6):
+        x.logits[b, int(x.lists[b][7])] = value
+    out = policy.preference_loss(*x.args(), lines, frozen)
+    for a, b in ((out.total, want.total), (out.loss, want.loss), (out.margin, want.margin), (out.line_logp, want.line_logp),
+                 (out.row_grad, want.row_grad)):
+        assert torch.equal(a, b)
+    assert (out.grad_logits[[1, 2, 5, 6]] == 0).all()
+    assert torch.equal(out.grad_logits[[0, 3, 4]], want.grad_logits[[0, 3, 4]])
+    # the clipped loss of a position without a played move likewise
+    one = torch.ones(7, device="cuda")
+    clip = policy.clipped_policy_loss(*x.args(), frozen, one, entropy_coef=0.1)
+    assert (clip.grad_logits[[1, 2]] == 0).all() and (clip.loss[[1, 2]] == 0).all()
