@@ -155,7 +155,8 @@ MFB200_API int mfb200_evaluate_priors(mfb200_handle *h, const uint64_t *masks, c
  * file, not the FastExp priors): move_logp [move_offsets[batch] -
  * move_offsets[0]], -inf past a position's 256th move; played_logp [batch] of
  * the played move, played[b] being its place in the position's list or -1 for
- * none (0 is returned); entropy [batch]. Lists as in mfb200_evaluate_priors;
+ * none (0 is returned, as for any place from 0 up where the list is empty);
+ * other places are refused; entropy [batch]. Lists as in mfb200_evaluate_priors;
  * any output may be NULL, and played where played_logp is; softmax_temp lies
  * between 1e-30 and 1e30. What a frozen
  * network contributes to the losses below. Blocks until the results are in
@@ -333,8 +334,8 @@ MFB200_API const char *mfb200_noalloc_last_error(void);
  * gradients, KL and entropy, log-probability 0 for its played move and -inf for
  * listed ones. A NaN or +inf among the listed logits makes the position's results
  * NaN. A position whose offsets decrease or reach outside [0, num_moves], or
- * whose played move is below -1 or not among its n moves, is not read past its
- * list: its per-position results and its whole gradient row are NaN. Sums and
+ * whose played move is below -1 or not among its n > 0 moves (where the list is
+ * empty any place from 0 up means none), is not read past its list: its per-position results and its whole gradient row are NaN. Sums and
  * softmax statistics are 32-bit or wider whatever the logits' type; each
  * gradient is rounded once to its own type. */
 

@@ -152,7 +152,7 @@ __device__ __forceinline__ Moves resolve(const PolicyRows &r, const ListHead &he
   m.lo = static_cast<int>(lo);
   m.count = m.bad ? 0 : static_cast<int>(hi - lo);
   m.n = min(m.count, kMaxMoves);
-  // a position with an empty list has no played move, whatever it is given
+  // a position with an empty list has no played move, whatever place (>= 0) it is given
   m.bad = m.bad || head.played < -1 || (m.count > 0 && head.played >= m.n);
   m.played = m.bad || m.count == 0 ? -1 : head.played;
   return m;

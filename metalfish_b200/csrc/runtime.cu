@@ -1943,7 +1943,8 @@ extern "C" int mfb200_evaluate_logprobs(mfb200_handle *h, const uint64_t *masks,
     if (move_offsets[b + 1] < move_offsets[b])
       return fail(h, "mfb200_evaluate_logprobs: move_offsets must be non-decreasing");
     const int64_t n = std::min<int64_t>(int64_t(move_offsets[b + 1]) - move_offsets[b], 256);
-    if (played && (played[b] < -1 || played[b] >= n))
+    // a position without moves has no played move, whatever place it is given (as in the operators)
+    if (played && (played[b] < -1 || (n > 0 && played[b] >= n)))
       return fail(h, "mfb200_evaluate_logprobs: played must be -1 or one of the position's first 256 moves");
   }
   const int nd = static_cast<int>(h->shards.size());
