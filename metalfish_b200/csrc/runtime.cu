@@ -33,7 +33,6 @@
 #include <mutex>
 #include <stdexcept>
 #include <string>
-#include <thread>
 #include <vector>
 
 #include "../../include/mfb200.h"
@@ -41,6 +40,7 @@
 #include "gemm_host.h"
 #include "kernels.cuh"
 #include "policy.cuh"
+#include "shards.h"
 
 using namespace mfb200;
 
@@ -1420,6 +1420,17 @@ int eval_shard(mfb200_handle *h, Shard &S, const uint64_t *masks, const float *v
   cudaEventElapsedTime(&ms[3], S.ev[0], S.ev[3]);
   return 0;
 }
+// work(i) for each of a handle's nd devices; the caller keeps its current device
+// where work that found no thread runs on the calling one.
+template <class Work>
+void on_shards(int nd, const Work &work) {
+  run_shards(nd, work, [&](int i) {
+    int device = -1;
+    const bool known = cudaGetDevice(&device) == cudaSuccess;
+    work(i);
+    if (known) cudaSetDevice(device);
+  });
+}
 // The forward followed by the legal-move priors of the shard's positions;
 // offsets/index/priors are the shard's slices of the caller's CSR arrays.
 int eval_shard_priors(mfb200_handle *h, Shard &S, const uint64_t *masks, const float *values,
@@ -1607,13 +1618,7 @@ extern "C" int mfb200_evaluate_history(mfb200_handle *h, const mfb200_board *boa
       errs[i] = e.what();
     }
   };
-  if (nd == 1) {
-    work(0);
-  } else {
-    std::vector<std::thread> th;
-    for (int i = 0; i < nd; ++i) th.emplace_back(work, i);
-    for (auto &t : th) t.join();
-  }
+  on_shards(nd, work);
   for (auto &e : errs)
     if (!e.empty()) return fail(h, "mfb200_evaluate_history: " + e);
   if (timing) {
@@ -1803,13 +1808,7 @@ int leaves_impl(mfb200_handle *h, const mfb200_board *boards, const int32_t *his
       errs[i] = e.what();
     }
   };
-  if (nd == 1) {
-    work(0);
-  } else {
-    std::vector<std::thread> th;
-    for (int i = 0; i < nd; ++i) th.emplace_back(work, i);
-    for (auto &t : th) t.join();
-  }
+  on_shards(nd, work);
   for (auto &e : errs)
     if (!e.empty()) return fail(h, std::string(fn) + ": " + e);
   if (timing) {
@@ -1901,13 +1900,7 @@ extern "C" int mfb200_evaluate_priors(mfb200_handle *h, const uint64_t *masks,
       errs[i] = e.what();
     }
   };
-  if (nd == 1) {
-    work(0);
-  } else {
-    std::vector<std::thread> th;
-    for (int i = 0; i < nd; ++i) th.emplace_back(work, i);
-    for (auto &t : th) t.join();
-  }
+  on_shards(nd, work);
   for (auto &e : errs)
     if (!e.empty()) return fail(h, "mfb200_evaluate_priors: " + e);
   if (timing) {
@@ -1973,17 +1966,7 @@ extern "C" int mfb200_evaluate_logprobs(mfb200_handle *h, const uint64_t *masks,
       errs[i] = e.what();
     }
   };
-  std::vector<std::thread> th;
-  th.reserve(nd);
-  for (int i = 1; i < nd; ++i) {
-    try {
-      th.emplace_back(work, i);
-    } catch (const std::exception &) {
-      work(i);  // no thread to be had
-    }
-  }
-  work(0);
-  for (auto &t : th) t.join();
+  on_shards(nd, work);
   for (auto &e : errs)
     if (!e.empty()) return fail(h, "mfb200_evaluate_logprobs: " + e);
   if (timing) {
@@ -2025,13 +2008,7 @@ extern "C" int mfb200_evaluate(mfb200_handle *h, const uint64_t *masks, const fl
       errs[i] = e.what();
     }
   };
-  if (nd == 1) {
-    work(0);
-  } else {
-    std::vector<std::thread> th;
-    for (int i = 0; i < nd; ++i) th.emplace_back(work, i);
-    for (auto &t : th) t.join();
-  }
+  on_shards(nd, work);
   for (auto &e : errs)
     if (!e.empty()) return fail(h, "mfb200_evaluate: " + e);
   if (timing) {

@@ -49,3 +49,18 @@ def test_played_move_of_a_position_without_moves(setup):
             net.evaluate_logprobs(inp, off, idx, bad)
         out = policy.move_logprobs(logits, *lists, torch.from_numpy(bad).cuda())
         assert torch.isnan(out.played).nonzero().flatten().cpu().tolist() == [b]
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_the_callers_device_stays_current(setup):
+    """A handle on two devices: each shard runs on a thread of its own."""
+    _, inp, off, idx = setup
+    pair = create_network(synthetic.TINY, synthetic.generate(synthetic.TINY, 11, perturb_norms=True), max_batch=B, num_devices=2)
+    try:
+        for device in (0, 1):
+            torch.cuda.set_device(device)
+            pair.evaluate_logprobs(inp, off, idx)
+            assert torch.cuda.current_device() == device
+    finally:
+        torch.cuda.set_device(0)
+        pair.close()
