@@ -329,15 +329,17 @@ MFB200_API const char *mfb200_noalloc_last_error(void);
  * softmax_temp, logp_j = s_j - log(sum exp s). An index outside [0, classes)
  * counts as logit 0 and gets no gradient; an index that is listed twice counts
  * twice, and its column gets the sum of both gradients. Columns that are not
- * listed are never read, whatever they hold. A position without a legal move
+ * listed have no effect, whatever they hold (column 0 of a position with moves may
+ * be loaded all the same, and is dropped). A position without a legal move
  * (empty list, or every listed logit -inf) takes part in nothing: zero losses,
  * gradients, KL and entropy, log-probability 0 for its played move and -inf for
  * listed ones. A NaN or +inf among the listed logits makes the position's results
  * NaN. A position whose offsets decrease or reach outside [0, num_moves], or
  * whose played move is below -1 or not among its n > 0 moves (where the list is
- * empty any place from 0 up means none), is not read past its list: its per-position results and its whole gradient row are NaN. Sums and
- * softmax statistics are 32-bit or wider whatever the logits' type; each
- * gradient is rounded once to its own type. */
+ * empty any place from 0 up means none), is not read past its list: its
+ * per-position results and its whole gradient row are NaN. Sums and softmax
+ * statistics are 32-bit or wider whatever the logits' type; each gradient is
+ * rounded once to its own type. */
 
 /* Element types of matrices of logits and of their gradients. */
 enum { MFB200_TYPE_F32 = 0, MFB200_TYPE_BF16 = 1, MFB200_TYPE_F16 = 2 };
