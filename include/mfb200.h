@@ -372,8 +372,10 @@ MFB200_API int mfb200_move_logprobs(const mfb200_policy_rows *rows, float *d_mov
  * grad_stride elements apart in grad_type. All columns are written (0 for
  * moves that are not listed); elements between the rows are left as they are.
  * With d_grad_moves = -target this is the gradient of the cross-entropy to a
- * distribution over the legal moves, such as the search's visit counts. The
- * gradient may not overlap an input. */
+ * distribution over the legal moves, such as the search's visit counts. A
+ * gradient that overlaps another array of its call is refused; it may lie in other
+ * columns of the same wide buffer as a matrix of the same row pitch in bytes, but
+ * no array may lie between its rows. */
 MFB200_API int mfb200_move_logprobs_backward(const mfb200_policy_rows *rows,
                                              const float *d_grad_moves, const float *d_grad_played,
                                              const float *d_grad_entropy, void *d_grad_logits,

@@ -1219,18 +1219,27 @@ int type_size(int type) {
 
 bool aligned(const void *p, int size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
 
-// Byte range of a [batch, classes] matrix whose rows are `stride` elements apart.
+// Bytes of an array, or of a [batch, classes] matrix whose rows are `stride`
+// elements apart. Matrices of one pitch may lie in one another's gaps (columns of
+// one wide buffer): they meet where their columns do.
 struct Range {
   uintptr_t lo, hi;
-  bool meets(const Range &o) const { return lo < o.hi && o.lo < hi; }
+  uintptr_t pitch, width;  // of a matrix, else 0
+  bool meets(const Range &o) const {
+    if (lo >= o.hi || o.lo >= hi) return false;
+    if (!pitch || pitch != o.pitch) return true;
+    const uintptr_t past = lo <= o.lo ? (o.lo - lo) % pitch : (pitch - (lo - o.lo) % pitch) % pitch;
+    return past < width || pitch - past < o.width;
+  }
 };
 Range matrix(const void *p, long long stride, int type, int batch, int classes) {
-  const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
-  return {lo, lo + (static_cast<uintptr_t>(batch - 1) * stride + classes) * type_size(type)};
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(p), pitch = static_cast<uintptr_t>(stride) * type_size(type),
+                  width = static_cast<uintptr_t>(classes) * type_size(type);
+  return {lo, lo + (batch - 1) * pitch + width, pitch, width};
 }
 Range array(const void *p, long long n, int size) {
   const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
-  return {lo, p ? lo + static_cast<uintptr_t>(n) * size : lo};
+  return {lo, p ? lo + static_cast<uintptr_t>(n) * size : lo, 0, 0};
 }
 
 const char *check_matrix(const void *p, long long stride, int type, int classes, int batch) {

@@ -165,3 +165,30 @@ def test_positions_that_take_no_part_have_no_gradient(value):
     one = torch.ones(7, device="cuda")
     clip = policy.clipped_policy_loss(*x.args(), frozen, one, entropy_coef=0.1)
     assert (clip.grad_logits[[1, 2]] == 0).all() and (clip.loss[[1, 2]] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("gap", [0, 1, 5])
+def test_gradient_in_the_logits_own_buffer(dtype, gap):
+    """Logits and gradient in columns of one wide buffer, the gradient's rows at any
+    alignment: as in buffers of their own, and nothing else is written."""
+    x = Batch(dtype, 301, [20, 70, 0, 33, 300] * 60, 47)
+    wide = torch.full((x.n, 2 * 301 + gap + 3), 7.0, dtype=x.logits.dtype, device="cuda")
+    wide[:, 1:302] = x.logits
+    before = wide.clone()
+    logits, grad = wide[:, 1:302], wide[:, 302 + gap:603 + gap]
+    rest = x.args()[1:]
+    one = torch.ones(x.n, device="cuda")
+    lines = torch.arange(0, x.n + 1, 10, dtype=torch.int32, device="cuda")
+    want = [policy.move_logprobs_backward(*x.args(), grad_played=one),
+            policy.clipped_policy_loss(*x.args(), one - 4, one, entropy_coef=0.1).grad_logits,
+            policy.preference_loss(*x.args(), lines[:31], one - 4).grad_logits]
+    calls = [lambda: policy.move_logprobs_backward(logits, *rest, grad_played=one, grad_logits=grad),
+             lambda: policy.clipped_policy_loss(logits, *rest, one - 4, one, entropy_coef=0.1, grad_logits=grad),
+             lambda: policy.preference_loss(logits, *rest, lines[:31], one - 4, grad_logits=grad)]
+    for call, g in zip(calls, want):
+        grad.fill_(7.0)
+        call()
+        assert torch.equal(grad, g)
+        wide[:, 302 + gap:603 + gap] = 7.0
+        assert torch.equal(wide, before)
