@@ -64,7 +64,7 @@ def clip64(r, old, adv, weight, ref, low, high, beta, eta, scale):
     old, adv, w = old.double(), adv.double(), weight.double() * scale
     lp = r.played_logp
     ratio = torch.exp(lp - old)
-    border = torch.where(adv > 0, 1 + high, 1 - low)
+    border = torch.full_like(adv, 1 - low).masked_fill_(adv > 0, 1 + high)  # (where() of two numbers is 32-bit)
     active = torch.where(adv > 0, ratio <= border, ratio >= border)
     kl = klm = torch.zeros_like(lp)
     delta, slack = torch.zeros_like(r.p), r.slack
