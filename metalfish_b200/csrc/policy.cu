@@ -119,8 +119,9 @@ __device__ __forceinline__ float exp2_fast(float t) {
   return v;
 }
 // e^s for s <= 0 as 2^(s log2 e), log2 e in two parts: the rounding of the
-// argument is that of one operation and does not lean to one side, which sums
-// of log-probabilities over long lines would add up.
+// argument is that of one operation and does not lean to one side, as it would over
+// the sum of a long list. (Log-probabilities of lines do without it: they are made
+// in 64 bits, line_position.)
 __device__ __forceinline__ float exp_fast(float s) {
   return exp2_fast(fmaf(s, kLog2e, s * kLog2eRest));
 }
@@ -850,7 +851,7 @@ struct ClipArgs {
 // KL = sum p (e^-d - 1 + d) with d = log p - log q (sum p e^-d = sum q = 1):
 // every term is >= 0 and an error common to all d cancels, so the KL of two
 // near policies keeps its digits. For |d| < 1/2 by the series d^2/2 - d^3/6 +
-// ... + d^8/8!, whose next term is 3e-8 of it; else from p, q and d themselves.
+// ... + d^8/8!, whose next term is at most 5e-8 of it; else from p, q and d themselves.
 __device__ __forceinline__ float kl_term(float p, float pr, float d) {
   float t = 1.0f / 40320;
   t = fmaf(t, -d, 1.0f / 5040);

@@ -192,3 +192,20 @@ def test_gradient_in_the_logits_own_buffer(dtype, gap):
         assert torch.equal(grad, g)
         wide[:, 302 + gap:603 + gap] = 7.0
         assert torch.equal(wide, before)
+
+
+def test_log_probabilities_of_lines_are_rounded_once():
+    """Made in 64 bits (100 steps of 2^-52 between kernel and oracle, per unit of
+    |s|, as where lines cancel) and rounded once: U |logp|. From 32-bit
+    exponentials they would be off by some U whatever |logp| is. One rounding to nearest leans
+    to neither side: errors of at most U |logp|, in the mean below a third of that
+    rms, leave U rms(logp) / sqrt(3 n); five times that is allowed."""
+    temp, n = 1.93, 1200
+    x = Batch("f32", 1858, [int(k) for k in np.random.default_rng(5).integers(2, 60, n)], 29, temp)
+    x.logits[:, :] *= 0.25  # log-probabilities of -0.2 to -5
+    rows, logp, frozen, lines = line_case(x, [0, 800, n])
+    out = policy.preference_loss(*x.args(), lines, x.f32(frozen), beta=0.1, softmax_temp=temp)
+    off = out.logp.double().cpu().numpy() - logp
+    tiny = 100 * 2.0 ** -52 * (1 + np.array([r.slack for r in rows]) / 8)
+    assert np.all(np.abs(off) <= ref.U * np.abs(logp) + tiny)
+    assert abs(off.mean()) <= 5 * ref.U * np.sqrt(np.mean(logp ** 2) / (3 * n))
