@@ -864,6 +864,13 @@ __device__ __forceinline__ float kl_term(float p, float pr, float d) {
   return p == 0.0f ? pr : fabsf(d) < 0.5f ? near : far;
 }
 
+// What the rounding of d = a - b leaves (the exact difference is d plus it); NaN
+// where one is infinite.
+__device__ __forceinline__ float difference_rest(float a, float b, float d) {
+  const float t = d - a;
+  return (a - (d - t)) - (b + t);
+}
+
 // Returns true, with nothing written, for a ratio too near the clip's border
 // to be decided in 32 bits, unless kExact.
 template <int G, bool kExact, int kType>
@@ -882,7 +889,6 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   if (a.ref) load_logits<G>(m.n, ref, ref_type, v.col, ref_bits);
   const float old = a.old_logp[b], adv = a.advantage[b];
   const float c = a.scale * (a.weight ? a.weight[b] : 1.0f);
-  const bool kl_counts = a.ref && a.kl_coef != 0.0f;  // 0 times an infinite KL is no term
   logits_of<G>(m.n, row, type, v.col, bits, v.z);
   if (a.ref) logits_of<G>(m.n, ref, ref_type, v.col, ref_bits, d);
   float es;
@@ -892,14 +898,16 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
     float er[G], es_r;
     Norm w = softmax_part<G>(m.n, d, r.inv_temp, lane, er, es_r);
     h = softmax_done<Sums::kSecond>(q, es, w, kl, lane);
+    const float tops = q.top - w.top;
+    const float tops_rest = difference_rest(q.top, w.top, tops);
 #pragma unroll
     for (int k = 0; k < G; ++k) {
       if (32 * k < m.n) {
-        // Both rows' gaps to their largest logit are nearly exact in 64 bits, and so is
-        // their difference: of near policies, and of logits with a number of their own
-        // added to each row (in 32 bits the two needs exclude each other).
-        const double gap = (static_cast<double>(v.z[k]) - q.top) - (static_cast<double>(d[k]) - w.top);
-        d[k] = static_cast<float>(gap) * r.inv_temp + (w.log_s - q.log_s);
+        // z - z' minus the difference of the tops, with what either rounding leaves: exact, for near
+        // policies and for logits with a number of their own added to each row
+        const float x = v.z[k] - d[k], low = difference_rest(v.z[k], d[k], x) - tops_rest;
+        const float apart = (x - tops) + (low == low ? low : 0.0f);
+        d[k] = apart * r.inv_temp + (w.log_s - q.log_s);
         kl += kl_term(v.e[k] * q.inv_s, er[k] * w.inv_s, d[k]);
       }
     }
@@ -910,8 +918,7 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   const bool takes = q.live && m.played >= 0;
   const float za = of_move<G>(v.z, m.played < 0 ? 0 : m.played, lane);
   const float sa = (za - q.top) * r.inv_temp;
-  float ratio = exp_fast((sa - old) - q.log_s);
-  if (adv == 0.0f && ratio == INFINITY) ratio = 1.0f;  // the surrogate is 0 for any ratio
+  const float ratio = exp_fast((sa - old) - q.log_s);
   // The gradient jumps where the ratio crosses the clip's border, so a ratio
   // within the rounding of the border is computed again in 64 bits.
   const float border = static_cast<float>(adv > 0.0f ? a.high : a.low);
@@ -928,8 +935,10 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
         exp((static_cast<double>(za) - q.top) / r.temp - log(sum) - static_cast<double>(old));
     active = adv > 0.0f ? !(exact > a.high) : !(exact < a.low);
   }
+  // A term whose coefficient is 0 (advantage, kl_coef) is left out: the ratio and the
+  // KL may be infinite. kl_coef is 0 without a reference.
   if (a.grad.base) {
-    const float slope = active ? -adv * ratio : 0.0f;
+    const float slope = active && adv != 0.0f ? -adv * ratio : 0.0f;
     float g[G];
 #pragma unroll
     for (int k = 0; k < G; ++k) {
@@ -937,7 +946,7 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
       const float p = v.e[k] * q.inv_s;
       float t = slope * played_term(m, q, 32 * k + lane, p);
       if (p != 0.0f) {
-        if (kl_counts) t += a.kl_coef * p * (d[k] - kl);
+        if (a.kl_coef != 0.0f) t += a.kl_coef * p * (d[k] - kl);
         t += a.entropy_coef * p * ((v.z[k] - q.top) * r.inv_temp - q.log_s + h);
       }
       g[k] = c * r.inv_temp * t;
@@ -947,8 +956,8 @@ __device__ __forceinline__ bool clip_position(const PolicyRows &r, const ClipArg
   }
   // after the row: the fence before its copy would wait for these stores
   if (lane == 0) {
-    float loss = -adv * (active ? ratio : border);
-    if (kl_counts) loss += a.kl_coef * kl;
+    float loss = adv != 0.0f ? -adv * (active ? ratio : border) : 0.0f;
+    if (a.kl_coef != 0.0f) loss += a.kl_coef * kl;
     loss -= a.entropy_coef * h;
     if (a.loss) a.loss[b] = takes ? c * loss : 0.0f;
     if (a.logp) a.logp[b] = takes ? sa - q.log_s : 0.0f;

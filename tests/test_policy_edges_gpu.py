@@ -209,3 +209,21 @@ def test_log_probabilities_of_lines_are_rounded_once():
     tiny = 100 * 2.0 ** -52 * (1 + np.array([r.slack for r in rows]) / 8)
     assert np.all(np.abs(off) <= ref.U * np.abs(logp) + tiny)
     assert abs(off.mean()) <= 5 * ref.U * np.sqrt(np.mean(logp ** 2) / (3 * n))
+
+
+@pytest.mark.parametrize("shift", [0.0, 3.0, 100.0, -65536.0])
+@pytest.mark.parametrize("near_by", [1e-3, 0.3])
+def test_kl_keeps_its_digits_at_any_offset(near_by, shift):
+    """Each d = log p - log q is good to a few U of itself and of the two
+    normalisations' difference, whose error is common to all d and cancels in sum p
+    (e^-d - 1 + d) to first order; the terms are positive, so the KL's relative
+    error is that of p, below slack U (policy_reference doubles it)."""
+    x = Batch("f32", 1858, [40, 64, 90, 2] * 16, 48)
+    _, other, old, adv, _ = clip_case(x, near_by=near_by)
+    x.logits = x.logits + shift
+    out = policy.clipped_policy_loss(*x.args(), x.f32(old), x.f32(adv), ref_logits=other, kl_coef=1.0)
+    for b, (p, q) in enumerate(zip(x.rows(), x.rows(other))):
+        # (from 64-bit differences of the logits: log p - log q loses half of the oracle's digits)
+        d = (p.z - q.z) - (p.z.max() - q.z.max()) + (q.log_s - p.log_s)
+        kl = np.sum(p.p * (np.expm1(-d) + d))
+        near(out.kl[b].item(), kl, p.slack * ref.U * kl, f"kl {b}")
