@@ -316,8 +316,9 @@ MFB200_API const char *mfb200_noalloc_last_error(void);
  * pointer of the current device (the logits' device is checked); the work is
  * enqueued on `stream` (a cudaStream_t, NULL = legacy default stream) without
  * synchronising. The calls allocate nothing, keep nothing between calls and
- * can be captured into a CUDA graph (make a first call on the device before); calls on different streams or threads do
- * not share anything but the buffers they are given. Results do not depend on
+ * can be captured into a CUDA graph (make a first call on the device before);
+ * calls on different streams or threads do not share anything but the buffers they
+ * are given. Results do not depend on
  * timing: the same inputs give the same bits. (The one exception: offsets that
  * decrease may put an entry of move_index into two lists, or a position into
  * the lines of two pairs; its move_logp entry or its gradient is then either
@@ -395,7 +396,9 @@ typedef struct {
  *             + kl_coef * KL - entropy_coef * H ),
  * KL = sum p (log p - log q) over the legal moves against the softmax q of
  * d_ref_logits ([batch, classes], rows ref_stride apart, ref_type; same
- * softmax_temp; NULL for no KL term), H the entropy. d_weight NULL means 1. A
+ * softmax_temp; NULL for no KL term), H the entropy. d_weight NULL means 1 (a weight
+ * of 0 is a factor like any other: a position whose numbers may not be finite is
+ * left out by having no played move). A
  * position without a played move has loss 0 and a zero gradient, whatever its
  * logits hold. An advantage of 0
  * makes the first term 0, also where the ratio overflows. The clip is

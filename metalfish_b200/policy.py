@@ -18,7 +18,8 @@ Common arguments: ``logits`` [batch, classes] float32, bfloat16 or float16,
 unit stride along a row; ``move_offsets`` int32 [batch + 1] and ``move_index``
 int16 [moves]; ``played`` int32 [batch], the played move's place in its
 position's list or -1; ``softmax_temp``. Gradients have the logits' type, or
-that of ``grad_logits`` where the caller gives the tensor to write.
+that of ``grad_logits`` where the caller gives the tensor to write (which may be
+other columns of the logits' own buffer).
 """
 from __future__ import annotations
 
@@ -185,7 +186,8 @@ _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream",
 def move_logprobs(logits, move_offsets, move_index, played=None, *,
                   softmax_temp: float = 1.0) -> MoveLogprobs:
     """Log-probabilities of the legal moves, of the played moves and the
-    entropy of each position (``mfb200_move_logprobs``)."""
+    entropy of each position (``mfb200_move_logprobs``). Entries of ``moves`` that
+    no position's list holds (a longer ``move_index``, a malformed list) are not set."""
     L = _lib()
     rows, shape, device = _rows(logits, move_offsets, move_index, played, softmax_temp)
     f = torch.float32
