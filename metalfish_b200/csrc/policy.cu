@@ -23,8 +23,8 @@
 // their SM and their warps take positions in turn, the lists of the next ones
 // loaded ahead. A gradient row is put together in shared memory and written by
 // one bulk copy, while the warp goes on. 65536 positions, 1858 fp32 classes, on
-// B200: clipped loss with KL 128 us (615 MB of DRAM traffic; the same reads and
-// copies without any arithmetic 127 us, the copies alone 92), the backward pass
+// B200: clipped loss with KL 128 us (617 MB of DRAM traffic; the same reads and
+// copies without any arithmetic 127-129 us, the copies alone 93), the backward pass
 // alone 110 us, log-probabilities 28 us.
 #include "policy.cuh"
 
@@ -57,7 +57,7 @@ constexpr float kLog2eRest = static_cast<float>(1.4426950408889634 - static_cast
 
 // The bits of a logit. L2 takes 64 bytes from DRAM for it instead of the 128
 // that a plain load takes: 65536 gathers of 16 pairs of logits a row read 88 MB
-// instead of 155, in 17.4 instead of 26.5 us.
+// instead of 155, in 16-17 instead of 26.6 us.
 __device__ __forceinline__ unsigned load_bits(const void *row, int type, int c) {
   if (type == MFB200_TYPE_F32) {
     unsigned v;
