@@ -119,9 +119,9 @@ __device__ __forceinline__ float exp2_fast(float t) {
   return v;
 }
 // e^s for s <= 0 as 2^(s log2 e), log2 e in two parts: the rounding of the
-// argument is that of one operation and does not lean to one side, as it would over
-// the sum of a long list. (Log-probabilities of lines do without it: they are made
-// in 64 bits, line_position.)
+// argument is that of one operation and does not lean to one side, which the sum of
+// a long list would add up. (Log-probabilities of lines are made in 64 bits instead,
+// line_position.)
 __device__ __forceinline__ float exp_fast(float s) {
   return exp2_fast(fmaf(s, kLog2e, s * kLog2eRest));
 }
